@@ -53,7 +53,8 @@ Type parse_type_text(const char* s) {
 // every node that launches kernels, the bodies of control nodes included, in program order
 void kernel_nodes(const std::vector<Node>& ns, std::vector<const Node*>& out) {
   for (auto& n : ns) {
-    if (n.kind == N_USE || n.kind == N_ACOND || n.kind == N_AWHILE || n.kind == N_APPLY || n.kind == N_ATRACE) {
+    if (n.kind == N_USE || n.kind == N_ACOND || n.kind == N_AWHILE || n.kind == N_APPLY || n.kind == N_ATRACE ||
+        (n.kind == N_AFOREIGN && n.foreign == F_NONE)) {
       for (auto& b : n.body) kernel_nodes(b.nodes, out);
     } else if (n.kind != N_RESHAPE) {
       out.push_back(&n);
@@ -65,7 +66,7 @@ void build_nodes(Program& p) {
   std::vector<const Node*> ks;
   kernel_nodes(p.ir->nodes, ks);
   for (const Node* n : ks) {
-    p.nodes[n->id].glue = build_glue(*n, p.ir->arrays);
+    p.nodes[n->id].glue = n->kind == N_AFOREIGN ? foreign_glue(*n) : build_glue(*n, p.ir->arrays);
     p.nodes[n->id].has_glue = true;
   }
 }

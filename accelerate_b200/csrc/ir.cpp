@@ -549,7 +549,7 @@ void parse_node(ProgramIR& p, std::vector<Node>& into, const Sx& bind, TEnv& env
   n.id = p.n_nodes++;
   const std::string k = x.head();
   // (control nodes are not hashed into any kernel: their text, which may embed whole arrays, is not kept)
-  if (k != "use" && k != "acond" && k != "awhile" && k != "apply" && k != "atrace") n.text = sx_text(x);
+  if (k != "use" && k != "acond" && k != "awhile" && k != "apply" && k != "atrace" && k != "aforeign") n.text = sx_text(x);
   auto is_operand = [](const Sx& s) { return s.head() == "manifest" || s.head() == "delayed"; };
   std::vector<ArrayInfo> outs;
   if (k == "generate") {
@@ -698,6 +698,27 @@ void parse_node(ProgramIR& p, std::vector<Node>& into, const Sx& bind, TEnv& env
     }
     if (!same_arrays(given, n.body[0].param_info)) throw Error(B200_ERR_TYPE, "apply: arguments do not match the function's parameters");
     outs = body_result(p, n.body[0]);
+  } else if (k == "aforeign") {
+    // (aforeign NAME (consts c..) (afun (x..) .. (out r..)) (args a..)): Aforeign (AST.hs:307-316).  The function is the
+    // definition in array code; it runs when no implementation is registered under NAME (Interpreter.hs:217).
+    n.kind = N_AFOREIGN;
+    if (!x.at(1).atom || x.at(2).head() != "consts" || x.at(4).head() != "args") throw Error(B200_ERR_PARSE, "expected (aforeign NAME (consts ...) (afun ...) (args ...))");
+    n.foreign = foreign_named(x.at(1).s);
+    for (size_t j = 1; j < x.at(2).size(); ++j) {
+      const std::string& c = x.at(2).k[j].s;
+      char* end = nullptr;
+      n.consts.push_back(strtod(c.c_str(), &end));
+      if (c.empty() || *end) throw Error(B200_ERR_PARSE, "aforeign: '" + c + "' is not a number");
+    }
+    n.body.push_back(parse_body(p, x.at(3), env, true));
+    const Sx& as = x.at(4);
+    for (size_t j = 1; j < as.size(); ++j) {
+      n.args.push_back(as.k[j].s);
+      n.arg_info.push_back(env.array(as.k[j].s));
+    }
+    if (!same_arrays(n.arg_info, n.body[0].param_info)) throw Error(B200_ERR_TYPE, "aforeign: arguments do not match the function's parameters");
+    outs = body_result(p, n.body[0]);
+    if (n.foreign != F_NONE) foreign_check(n, outs);
   } else if (k == "atrace") {
     // (atrace (hex MESSAGE) (show a..) (args b..)): Atrace, Interpreter.hs:215 -- print the message and the
     // arrays a.., hand the arrays b.. on unchanged

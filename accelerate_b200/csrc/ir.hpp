@@ -170,7 +170,10 @@ struct BoundarySpec {
 // Use (a constant array embedded in the program), Acond, Awhile and Apply, whose operands are
 // array-level functions (`Body`).
 enum NodeKind { N_GENERATE, N_FOLD, N_FOLDSEG, N_SCAN, N_SCAN2, N_PERMUTE, N_STENCIL, N_STENCIL2, N_RESHAPE,
-                N_USE, N_ACOND, N_AWHILE, N_APPLY, N_ATRACE };
+                N_USE, N_ACOND, N_AWHILE, N_APPLY, N_ATRACE, N_AFOREIGN };
+// Array functions this backend has an implementation of its own for (Aforeign, AST.hs:307-316): rows.cpp.
+// F_NONE: the node's pure fallback is applied (Interpreter.hs:217).
+enum Foreign { F_NONE, F_LOG_PROBS, F_DISTILL, F_DISTILL_GRAD, F_LAYER_NORM, F_LAYER_NORM_GRAD };
 struct Node;
 // An array-level function or a branch: parameters (none for branches), nodes, results.
 struct Body {
@@ -182,10 +185,13 @@ struct Body {
 struct Node {
   NodeKind kind = N_GENERATE;
   int id = -1;                            // position in Program::nodes (unique over all bodies)
-  std::vector<Body> body;                 // acond: then, else; awhile: condition, step; apply: the function
-  std::vector<std::string> args;          // awhile: initial state; apply: arguments; atrace: the arrays handed on
+  std::vector<Body> body;                 // acond: then, else; awhile: condition, step; apply, aforeign: the function
+  std::vector<std::string> args;          // awhile: initial state; apply, aforeign: arguments; atrace: the arrays handed on
   std::vector<std::string> shown;         // atrace: the arrays to print
   std::string message;                    // atrace
+  Foreign foreign = F_NONE;               // aforeign: the implementation found under its name
+  std::vector<double> consts;             // aforeign: constants of the implementation
+  std::vector<ArrayInfo> arg_info;        // aforeign: ranks and element types of the arguments
   std::unique_ptr<Expr> pred;             // acond
   std::vector<int64_t> use_shape;         // use
   std::vector<std::string> use_data;      // use: raw bytes of every scalar leaf
@@ -221,6 +227,9 @@ std::string program_text_lowered(const char* text, size_t len);
 // Free array variables of an expression / function (names, in first-use order).
 void free_arrays(const Expr& e, std::vector<std::string>& out);
 void free_arrays(const Fun& f, std::vector<std::string>& out);
+// The implementation registered under a name, and its check of a node's constants, arguments and results (throws).
+Foreign foreign_named(const std::string& name);
+void foreign_check(const Node& n, const std::vector<ArrayInfo>& outs);
 // Every array variable a node mentions, the bodies of control nodes included.
 void node_arrays(const Node& n, std::vector<std::string>& out);
 

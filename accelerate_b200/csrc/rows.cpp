@@ -1,0 +1,354 @@
+// Foreign array functions of this backend (Aforeign, AST.hs:307-316; the reference's way to put hand-written code
+// behind an array function, with a definition in array code beside it): the row operators.
+//
+// Names, constants, arguments and results (sh: any outer shape, the same for all arguments of a call; t: Half or Float):
+//   b200.logProbs       (consts k)    tokens (sh, Int32 or Int), logits (sh:.n, t)
+//                                     -> (sh, (log probability, normaliser, entropy) Floats), (sh:.k, (Int32 index, Float))
+//   b200.distill        (consts tau)  ids (sh:.k, Int32), teacher (sh:.k, t'), student (sh:.n, t) -> (sh, loss), (sh, normaliser)
+//   b200.distillGrad    (consts tau)  ids, teacher, student, normaliser (sh, Float), gradient (sh, Float) -> (sh:.n, t)
+//   b200.layerNorm      (consts eps)  gamma, beta (Vector of t or Float), xs (sh:.n, t) -> (sh:.n, t), (sh, (mean, rstd) Floats)
+//   b200.layerNormGrad  (consts)      gamma, xs, (sh, (mean, rstd)), dys (sh:.n, t) -> (sh:.n, t), dgamma, dbeta (gamma's type)
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+
+#include "runtime.hpp"
+
+namespace accb200 {
+
+namespace {
+
+const struct { const char* name; Foreign op; } kForeign[] = {
+    {"b200.logProbs", F_LOG_PROBS},   {"b200.distill", F_DISTILL},           {"b200.distillGrad", F_DISTILL_GRAD},
+    {"b200.layerNorm", F_LAYER_NORM}, {"b200.layerNormGrad", F_LAYER_NORM_GRAD},
+};
+// the alternatives of logProbs: the list is selected and merged by one thread per entry
+constexpr int kMostAlternatives = 128;
+// indices inside a row are 32 bits (rows of a tile's width below 2^31)
+constexpr int64_t kMostColumns = (1LL << 31) - (1LL << 20);
+
+typedef std::map<std::string, std::string> Variant;
+
+bool is(const ArrayInfo& a, int rank, Ty t) { return a.rank == rank && !a.elt.tuple && a.elt.s == t; }
+bool is_real(const ArrayInfo& a) { return !a.elt.tuple && (a.elt.s == F16 || a.elt.s == F32); }
+bool is_floats(const ArrayInfo& a, int rank, size_t n) {
+  if (a.rank != rank || !a.elt.tuple || a.elt.e.size() != n) return false;
+  for (auto& c : a.elt.e)
+    if (c.tuple || c.s != F32) return false;
+  return true;
+}
+// the array of logits, or the rows to be normalised
+const ArrayInfo& rows_arg(const Node& n) {
+  switch (n.foreign) {
+    case F_LOG_PROBS: case F_LAYER_NORM_GRAD: return n.arg_info[1];
+    default: return n.arg_info[2];
+  }
+}
+std::string ctype(Ty t) { return t == F16 ? "u16" : t == F32 ? "f32" : t == I64 ? "i64" : "i32"; }
+std::string str(int64_t v) { return std::to_string(v); }
+
+}  // namespace
+
+Foreign foreign_named(const std::string& name) {
+  for (auto& f : kForeign)
+    if (name == f.name) return f.op;
+  return F_NONE;
+}
+
+void foreign_check(const Node& n, const std::vector<ArrayInfo>& outs) {
+  std::string name;
+  for (auto& f : kForeign)
+    if (f.op == n.foreign) name = f.name;
+  auto need = [&](bool ok, const std::string& what) { if (!ok) throw Error(B200_ERR_TYPE, name + ": " + what); };
+  const std::vector<ArrayInfo>& a = n.arg_info;
+  const size_t nargs[] = {0, 2, 3, 5, 3, 4}, nouts[] = {0, 2, 2, 1, 2, 3}, nconsts[] = {0, 1, 1, 1, 1, 0};
+  need(a.size() == nargs[n.foreign], "takes " + std::to_string(nargs[n.foreign]) + " arrays");
+  need(n.consts.size() == nconsts[n.foreign], "takes " + std::to_string(nconsts[n.foreign]) + " constants");
+  const ArrayInfo& x = rows_arg(n);
+  need(x.rank >= 1 && is_real(x), "the rows must be an array of Half or Float of rank 1 or more");
+  const int r = x.rank;
+  need(outs.size() == nouts[n.foreign], "the function yields another number of arrays");
+  switch (n.foreign) {
+    case F_LOG_PROBS: {
+      const double k = n.consts[0];
+      if (!(k >= 0 && k <= kMostAlternatives && k == std::floor(k)))
+        throw Error(B200_ERR_UNSUPPORTED, name + ": the number of alternatives must be a whole number from 0 to " + str(kMostAlternatives));
+      need(is(a[0], r - 1, I32) || is(a[0], r - 1, I64), "the given tokens must be Int32 or Int, one per row");
+      need(is_floats(outs[0], r - 1, 3) && outs[1].rank == r && outs[1].elt == Type::tup({Type::scalar(I32), Type::scalar(F32)}), "the function yields other arrays");
+      break;
+    }
+    case F_DISTILL: case F_DISTILL_GRAD: {
+      const double tau = n.consts[0];
+      // (outside this range products of the temperature and a Float logit leave the type's range)
+      if (!(tau >= 1e-4 && tau <= 1e4)) throw Error(B200_ERR_ARG, name + ": the temperature must lie between 1e-4 and 1e4");
+      need(is(a[0], r, I32), "the teacher's tokens must be Int32, one list per row");
+      need(a[1].rank == r && is_real(a[1]), "the teacher's logits must be Half or Float, one list per row");
+      if (n.foreign == F_DISTILL) {
+        need(is(outs[0], r - 1, F32) && is(outs[1], r - 1, F32), "the function yields other arrays");
+      } else {
+        need(is(a[3], r - 1, F32) && is(a[4], r - 1, F32), "normaliser and gradient must be Float, one per row");
+        need(is(outs[0], r, x.elt.s), "the function yields other arrays");
+      }
+      break;
+    }
+    case F_LAYER_NORM: {
+      if (!(n.consts[0] >= 0 && n.consts[0] <= 3.4e38)) throw Error(B200_ERR_ARG, name + ": epsilon must be finite and not negative");
+      need((is(a[0], 1, x.elt.s) || is(a[0], 1, F32)) && is(a[1], 1, a[0].elt.s), "gamma and beta must be vectors of the rows' type or of Float");
+      need(is(outs[0], r, x.elt.s) && is_floats(outs[1], r - 1, 2), "the function yields other arrays");
+      break;
+    }
+    case F_LAYER_NORM_GRAD:
+      need(is(a[0], 1, x.elt.s) || is(a[0], 1, F32), "gamma must be a vector of the rows' type or of Float");
+      need(is_floats(a[2], r - 1, 2), "the statistics must be pairs of Floats, one per row");
+      need(is(a[3], r, x.elt.s), "the gradient must have the rows' type and rank");
+      need(is(outs[0], r, x.elt.s) && is(outs[1], 1, a[0].elt.s) && is(outs[2], 1, a[0].elt.s), "the function yields other arrays");
+      break;
+    case F_NONE: break;
+  }
+}
+
+Glue foreign_glue(const Node& n) {
+  Glue g;
+  g.defines["ROW_F16"] = rows_arg(n).elt.s == F16 ? "1" : "0";
+  switch (n.foreign) {
+    case F_LOG_PROBS:
+      g.defines["ROW_DISTILL"] = "0";
+      g.defines["ROW_TOPK"] = n.consts[0] > 0 ? "1" : "0";
+      g.code = "typedef " + ctype(n.arg_info[0].elt.s) + " token_t;\n";
+      break;
+    case F_DISTILL:
+      g.defines["ROW_DISTILL"] = "1";
+      g.defines["ROW_TOPK"] = "0";
+      g.code = "typedef " + ctype(n.arg_info[1].elt.s) + " teacher_t;\n";
+      break;
+    case F_DISTILL_GRAD: g.code = "typedef " + ctype(n.arg_info[1].elt.s) + " teacher_t;\n"; break;
+    case F_LAYER_NORM: case F_LAYER_NORM_GRAD: g.code = "typedef " + ctype(n.arg_info[0].elt.s) + " param_t;\n"; break;
+    case F_NONE: break;
+  }
+  return g;
+}
+
+// ---- launch shapes ------------------------------------------------------------------------------------
+namespace {
+
+constexpr int kThreads = 256;
+
+Variant stats_variant(int ctas) { return {{"ROW_THREADS", str(kThreads)}, {"ROW_U", "4"}, {"ROW_MIN_BLOCKS", "3"}, {"ROW_C", str(ctas)}}; }
+Variant distill_grad_variant(int ctas) { return {{"ROW_THREADS", str(kThreads)}, {"ROW_U", "4"}, {"ROW_MIN_BLOCKS", "4"}, {"ROW_C", str(ctas)}}; }
+
+// CTAs that share a row: enough to give every SM several, as long as each has a tile of its own
+int ctas_per_row(int64_t rows, int64_t n, int elt_bytes, int sms, int most) {
+  const int64_t tiles = (n * elt_bytes + 16 * kThreads * 4 - 1) / (16 * kThreads * 4);
+  int c = 1;
+  while (c < most && rows * c < 8 * (int64_t)sms && 2 * c <= tiles) c *= 2;
+  return c;
+}
+
+// A row over warps and registers (rows_norm_pre.cuh)
+struct NormShape {
+  int ve, warps, u, threads;
+  bool whole;              // the row fits the registers
+  Variant variant() const {
+    return {{"ROW_THREADS", str(threads)}, {"NORM_VE", str(ve)}, {"NORM_WARPS", str(warps)}, {"NORM_U", str(u)}, {"NORM_LONG", whole ? "0" : "1"}};
+  }
+  int rows() const { return threads / 32 / warps; }
+};
+// the next size of the list 1 2 3 4 6 8 12 16 ...: few kernels for all lengths
+int round_up_u(int64_t u) {
+  int v = 1;
+  while (v < u) v = (v & (v - 1)) == 0 && v > 1 ? v + v / 2 : (v == 1 ? 2 : v / 3 * 4);
+  return v;
+}
+NormShape norm_shape(int64_t n, int ve, int most_elems, int most_warps, int64_t rows, int sms) {
+  NormShape s{ve, 1, 1, kThreads, true};
+  const int64_t units = std::max<int64_t>((n + ve - 1) / ve, 1);
+  const int most_u = std::max(1, most_elems / ve);
+  auto need = [&](int w) { return (units + w * 32 - 1) / (w * 32); };
+  while (s.warps < most_warps && need(s.warps) > most_u) s.warps *= 2;
+  // few rows: more warps on each, so that the machine has something to do
+  while (s.warps < 8 && need(s.warps) > 1 && rows * s.warps < 16 * (int64_t)sms) s.warps *= 2;
+  if (need(s.warps) > most_u) {
+    s.whole = false;
+    s.warps = 16;
+    s.u = 1;
+  } else {
+    s.u = round_up_u(need(s.warps));
+  }
+  s.threads = std::max(kThreads, s.warps * 32);
+  return s;
+}
+constexpr int kNormElems = 32, kNormWarps = 32;          // forward: elements per thread, warps per row
+constexpr int kNormGradElems = 16, kNormGradWarps = 16;
+
+}  // namespace
+
+std::vector<std::pair<std::string, Variant>> foreign_variants(const Node& n) {
+  std::vector<std::pair<std::string, Variant>> v;
+  const int ve = rows_arg(n).elt.s == F16 ? 8 : 4;
+  auto with = [](Variant a, const char* key) { a["NORM_SUMS"] = a["NORM_COLS"] = "0"; if (*key) a[key] = "1"; return a; };
+  switch (n.foreign) {
+    case F_LOG_PROBS: case F_DISTILL:
+      for (int c : {1, 4}) v.push_back({"rows_stats", stats_variant(c)});
+      break;
+    case F_DISTILL_GRAD: v.push_back({"rows_distill_grad", distill_grad_variant(1)}); break;
+    case F_LAYER_NORM:
+      for (int64_t len : {1024, 4096, 1 << 20})
+        for (int w : {ve, 1}) v.push_back({"rows_norm", norm_shape(len, w, kNormElems, kNormWarps, 1 << 20, 148).variant()});
+      break;
+    case F_LAYER_NORM_GRAD:
+      for (int64_t len : {1024, 4096, 1 << 20})
+        for (int w : {ve, 1}) v.push_back({"rows_norm_grad", with(norm_shape(len, w, kNormGradElems, kNormGradWarps, 1 << 20, 148).variant(), "")});
+      v.push_back({"rows_norm_grad", with(norm_shape(1, 1, 1, 1, 1, 1).variant(), "NORM_SUMS")});
+      v.push_back({"rows_norm_grad", with(norm_shape(1, 1, 1, 1, 1, 1).variant(), "NORM_COLS")});
+      break;
+    case F_NONE: break;
+  }
+  return v;
+}
+
+// ---- execution -------------------------------------------------------------------------------------------
+namespace {
+
+uint64_t ptr_of(const DevArray& a, int leaf = 0) { return (uint64_t)(uintptr_t)a.leaf[leaf]->ptr; }
+uint64_t float_bits(double v) {
+  const float f = (float)v;
+  uint32_t b;
+  memcpy(&b, &f, 4);
+  return b;
+}
+void launch(Ctx& c, CompiledKernel& k, int64_t grid, int threads, size_t smem, std::vector<uint64_t> params) {
+  if (grid <= 0) return;
+  if (grid > 2147483647LL) throw Error(B200_ERR_UNSUPPORTED, "grid too large");
+  void* args[1] = {params.data()};
+  c.check(c.drv.LaunchKernel(k.fn, (unsigned)grid, 1, 1, (unsigned)threads, 1, 1, (unsigned)smem, (CUstream)c.stream, args, nullptr), "cuLaunchKernel");
+  c.launches++;
+}
+
+}  // namespace
+
+void Program::exec_foreign(const Node& n, Env& env) {
+  Ctx& c = *ctx;
+  // Results and scratch come from the context's pool and go back to it when the caller frees them: a captured graph
+  // would keep writing to memory that belongs to somebody else by the time it is replayed.
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  c.check(cudaStreamIsCapturing(c.stream, &capture), "cudaStreamIsCapturing");
+  if (capture != cudaStreamCaptureStatusNone) throw Error(B200_ERR_UNSUPPORTED, "a row operator cannot be captured into a CUDA graph");
+  NodeState& st = nodes[n.id];
+  std::vector<DevArrayP> a;
+  for (auto& name : n.args) a.push_back(env.at(name));
+  const DevArray& x = *a[n.foreign == F_LOG_PROBS || n.foreign == F_LAYER_NORM_GRAD ? 1 : 2];
+  const std::vector<int64_t> outer(x.shape.begin(), x.shape.end() - 1);
+  const int64_t cols = std::max<int64_t>(x.shape.back(), 0);
+  int64_t rows = 1;
+  for (int64_t d : outer) rows *= std::max<int64_t>(d, 0);
+  if (cols > kMostColumns) throw Error(B200_ERR_UNSUPPORTED, "rows of " + str(cols) + " elements are too long");
+  auto outer_is = [&](const DevArray& b, bool list) {
+    if (std::vector<int64_t>(b.shape.begin(), b.shape.end() - (list ? 1 : 0)) != outer) throw Error(B200_ERR_BOUNDS, "shape mismatch");
+  };
+  const int elt_bytes = ty_bytes[x.elt.s];
+  const uint64_t err = (uint64_t)(uintptr_t)(c.d_words + 0);
+  switch (n.foreign) {
+    case F_LOG_PROBS: {
+      outer_is(*a[0], false);
+      const int64_t k = (int64_t)n.consts[0];
+      std::vector<int64_t> list = outer;
+      list.push_back(k);
+      DevArrayP stats = c.new_array(n.out_info[0].elt, outer), top = c.new_array(n.out_info[1].elt, list);
+      env[n.outs[0]] = stats;
+      env[n.outs[1]] = top;
+      if (rows == 0) break;
+      const int ctas = ctas_per_row(rows, cols, elt_bytes, c.sm_count, 8);
+      CompiledKernel& ker = node_kernel(c, st, "rows_stats", stats_variant(ctas), "acc_rows_stats", kThreads, 0);
+      launch(c, ker, rows * ctas, kThreads, 0,
+             {ptr_of(x), ptr_of(*a[0]), 0, ptr_of(*stats, 0), ptr_of(*stats, 1), ptr_of(*stats, 2), ptr_of(*top, 0), ptr_of(*top, 1),
+              (uint64_t)rows, (uint64_t)cols, (uint64_t)k, float_bits(1.0), err});
+      break;
+    }
+    case F_DISTILL: case F_DISTILL_GRAD: {
+      outer_is(*a[0], true);
+      outer_is(*a[1], true);
+      if (a[0]->shape != a[1]->shape) throw Error(B200_ERR_BOUNDS, "shape mismatch");
+      const int64_t k = std::max<int64_t>(a[0]->shape.back(), 0);
+      if (k > kMostColumns) throw Error(B200_ERR_UNSUPPORTED, "lists of " + str(k) + " teacher entries are too long");
+      if (n.foreign == F_DISTILL) {
+        DevArrayP loss = c.new_array(n.out_info[0].elt, outer), lse = c.new_array(n.out_info[1].elt, outer);
+        env[n.outs[0]] = loss;
+        env[n.outs[1]] = lse;
+        if (rows == 0) break;
+        const int ctas = ctas_per_row(rows, cols, elt_bytes, c.sm_count, 8);
+        CompiledKernel& ker = node_kernel(c, st, "rows_stats", stats_variant(ctas), "acc_rows_stats", kThreads, 0);
+        launch(c, ker, rows * ctas, kThreads, 0,
+               {ptr_of(x), ptr_of(*a[0]), ptr_of(*a[1]), ptr_of(*loss), ptr_of(*lse), 0, 0, 0, (uint64_t)rows, (uint64_t)cols, (uint64_t)k,
+                float_bits(n.consts[0]), err});
+      } else {
+        outer_is(*a[3], false);
+        outer_is(*a[4], false);
+        DevArrayP dx = c.new_array(n.out_info[0].elt, x.shape);
+        env[n.outs[0]] = dx;
+        if (rows == 0 || cols == 0) break;
+        const int ctas = ctas_per_row(rows, cols, elt_bytes, c.sm_count, 16);
+        CompiledKernel& ker = node_kernel(c, st, "rows_distill_grad", distill_grad_variant(ctas), "acc_rows_distill_grad", kThreads, 0);
+        launch(c, ker, rows * ctas, kThreads, 0,
+               {ptr_of(x), ptr_of(*a[0]), ptr_of(*a[1]), ptr_of(*a[3]), ptr_of(*a[4]), ptr_of(*dx), (uint64_t)rows, (uint64_t)cols, (uint64_t)k,
+                float_bits(n.consts[0]), err});
+      }
+      break;
+    }
+    case F_LAYER_NORM: {
+      if (a[0]->shape[0] != x.shape.back() || a[1]->shape[0] != x.shape.back()) throw Error(B200_ERR_BOUNDS, "shape mismatch");
+      DevArrayP y = c.new_array(n.out_info[0].elt, x.shape), stats = c.new_array(n.out_info[1].elt, outer);
+      env[n.outs[0]] = y;
+      env[n.outs[1]] = stats;
+      if (rows == 0) break;
+      const bool wide = x.aligned16() && y->aligned16() && a[0]->aligned16() && a[1]->aligned16() && cols * elt_bytes % 16 == 0;
+      const NormShape s = norm_shape(cols, wide ? 16 / elt_bytes : 1, kNormElems, kNormWarps, rows, c.sm_count);
+      CompiledKernel& ker = node_kernel(c, st, "rows_norm", s.variant(), "acc_rows_norm", s.threads, 0);
+      launch(c, ker, (rows + s.rows() - 1) / s.rows(), s.threads, 0,
+             {ptr_of(x), ptr_of(*a[0]), ptr_of(*a[1]), ptr_of(*y), ptr_of(*stats, 0), ptr_of(*stats, 1), (uint64_t)rows, (uint64_t)cols, float_bits(n.consts[0])});
+      break;
+    }
+    case F_LAYER_NORM_GRAD: {
+      if (a[0]->shape[0] != x.shape.back() || a[3]->shape != x.shape) throw Error(B200_ERR_BOUNDS, "shape mismatch");
+      outer_is(*a[2], false);
+      DevArrayP dx = c.new_array(n.out_info[0].elt, x.shape);
+      DevArrayP dgamma = c.new_array(n.out_info[1].elt, a[0]->shape), dbeta = c.new_array(n.out_info[2].elt, a[0]->shape);
+      env[n.outs[0]] = dx;
+      env[n.outs[1]] = dgamma;
+      env[n.outs[2]] = dbeta;
+      if (cols == 0) break;
+      const bool wide = x.aligned16() && dx->aligned16() && a[3]->aligned16() && a[0]->aligned16() && cols * elt_bytes % 16 == 0;
+      const NormShape s = norm_shape(cols, wide ? 16 / elt_bytes : 1, kNormGradElems, kNormGradWarps, rows, c.sm_count);
+      Variant var = s.variant();
+      var["NORM_SUMS"] = var["NORM_COLS"] = "0";
+      const size_t smem = s.whole && s.rows() > 1 ? (size_t)cols * 8 : 0;
+      CompiledKernel& ker = node_kernel(c, st, "rows_norm_grad", var, "acc_rows_norm_grad", s.threads, smem);
+      const int64_t grid = std::min<int64_t>((rows + s.rows() - 1) / s.rows(), (int64_t)c.sm_count * ker.max_blocks_per_sm);
+      // lines of partial sums: one per CTA; for long rows one per `chunk` rows
+      const int64_t tiles = (cols + 31) / 32;
+      int64_t lines = grid, chunk = 0;
+      if (!s.whole) {
+        chunk = std::max<int64_t>(8, (rows * tiles + 8 * c.sm_count - 1) / (8 * c.sm_count));
+        lines = (rows + chunk - 1) / chunk;
+      }
+      std::shared_ptr<Buffer> partial = c.alloc((size_t)lines * 2 * cols * 4);
+      const std::vector<uint64_t> params = {ptr_of(x), ptr_of(*a[0]), ptr_of(*a[2], 0), ptr_of(*a[2], 1), ptr_of(*a[3]), ptr_of(*dx),
+                                            (uint64_t)(uintptr_t)partial->ptr, ptr_of(*dgamma), ptr_of(*dbeta), (uint64_t)rows, (uint64_t)cols, (uint64_t)lines, (uint64_t)chunk};
+      launch(c, ker, grid, s.threads, smem, params);
+      Variant sums = norm_shape(1, 1, 1, 1, 1, 1).variant();
+      sums["NORM_SUMS"] = "0";
+      sums["NORM_COLS"] = "1";
+      if (!s.whole) {
+        CompiledKernel& kc = node_kernel(c, st, "rows_norm_grad", sums, "acc_rows_norm_cols", kThreads, 0);
+        launch(c, kc, lines * tiles, kThreads, 0, params);
+      }
+      sums["NORM_SUMS"] = "1";
+      sums["NORM_COLS"] = "0";
+      CompiledKernel& ks = node_kernel(c, st, "rows_norm_grad", sums, "acc_rows_norm_sums", kThreads, 0);
+      launch(c, ks, tiles, kThreads, 0, params);
+      break;
+    }
+    case F_NONE: break;
+  }
+}
+
+}  // namespace accb200

@@ -259,7 +259,10 @@ std::string assemble_source(const Glue& g, const std::string& skeleton, const st
   o << prelude_source() << "\n";
   if (skeleton == "stencil") o << skeleton_source("stencil_pre") << "\n";
   if (skeleton == "stencil2d") o << skeleton_source("stencil2d_pre") << "\n";
-  o << g.code << "\n" << skeleton_source(skeleton) << "\n";
+  o << g.code << "\n";
+  if (skeleton.compare(0, 5, "rows_") == 0) o << skeleton_source("rows_pre") << "\n";
+  if (skeleton.compare(0, 9, "rows_norm") == 0) o << skeleton_source("rows_norm_pre") << "\n";
+  o << skeleton_source(skeleton) << "\n";
   return o.str();
 }
 
@@ -400,6 +403,7 @@ std::vector<std::pair<std::string, std::map<std::string, std::string>>> default_
         }
       }
       break;
+    case N_AFOREIGN: return foreign_variants(n);
     default: break;   // reshape and the host-evaluated nodes launch nothing
   }
   return v;
@@ -905,6 +909,13 @@ void Program::exec(const std::vector<Node>& ns, Env& env) {
         for (size_t k = 0; k < n.outs.size(); ++k) env[n.outs[k]] = state[k];
         break;
       }
+      case N_AFOREIGN:
+        if (n.foreign != F_NONE) {
+          exec_foreign(n, env);
+          break;
+        }
+        // no implementation of that name: the fallback (Interpreter.hs:217)
+        // fall through
       case N_APPLY: {
         std::vector<DevArrayP> args;
         for (auto& a : n.args) args.push_back(env.at(a));
@@ -931,7 +942,7 @@ void Program::exec(const std::vector<Node>& ns, Env& env) {
 // The kernel of one node for one variant.  Assembling the source text and hashing it (what Ctx::kernel
 // keys on) costs tens of microseconds, too much for every launch of a program that runs many small
 // kernels, so a node remembers the kernels it has asked for by skeleton, entry point and variant.
-static CompiledKernel& node_kernel(Ctx& c, NodeState& st, const char* skeleton, const std::map<std::string, std::string>& variant, const char* entry,
+CompiledKernel& node_kernel(Ctx& c, NodeState& st, const char* skeleton, const std::map<std::string, std::string>& variant, const char* entry,
                                    int threads, size_t smem) {
   std::string key = skeleton;
   key += '|';

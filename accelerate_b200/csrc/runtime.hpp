@@ -170,8 +170,16 @@ struct Program {
   void liveness_of(const std::vector<Node>& nodes, const std::vector<std::string>& keep);
   void exec(const std::vector<Node>& nodes, Env& env);
   void exec_kernel_node(const Node& n, Env& env);
+  void exec_foreign(const Node& n, Env& env);        // rows.cpp
   std::vector<DevArrayP> call(const Body& b, const std::vector<DevArrayP>& args, Env& env);
 };
+
+// The kernel of one node for one variant, remembered in the node's state.
+CompiledKernel& node_kernel(Ctx& c, NodeState& st, const char* skeleton, const std::map<std::string, std::string>& variant, const char* entry,
+                            int threads, size_t smem);
+// The generated part of a foreign node's kernels (types only), and variants for the compile check: (skeleton, defines).
+Glue foreign_glue(const Node& n);
+std::vector<std::pair<std::string, std::map<std::string, std::string>>> foreign_variants(const Node& n);
 
 // Source text of one kernel variant: prelude, defines, generated code, skeleton.
 std::string assemble_source(const Glue& g, const std::string& skeleton, const std::map<std::string, std::string>& variant);

@@ -1,0 +1,213 @@
+// Gradients of layer norm (rows_norm.cuh).  With xh = (x - mu) r and a = dy gamma:
+//   dx = r (a - mean a - xh mean(a xh)),   dgamma = sum over rows of dy xh,   dbeta = sum over rows of dy.
+// Bound by HBM: x and dy are read once, dx is written once.  A CTA walks over rows NORM_ROWS at a time; a lane holds
+// the same columns of every row, so that the sums over rows stay in its registers.  At the end the CTA's sums go to
+// `partial` (one line of 2 n Floats per CTA) and acc_rows_norm_sums adds the lines in their order: the same
+// numbers every time, whatever order the CTAs ran in.
+// NORM_LONG: rows longer than the registers hold; dx alone (three reads of the row), the sums over rows by
+// acc_rows_norm_cols.
+
+struct Params { i64 x, gamma, mean, rstd, dy, dx, partial, dgamma, dbeta, rows, n, lines, chunk; };
+
+#if NORM_SUMS
+// Lines of partial sums -> dgamma, dbeta.  32 columns per CTA, the warps take lines in turn.
+extern "C" __global__ void __launch_bounds__(ROW_THREADS) acc_rows_norm_sums(const __grid_constant__ Params p) {
+  __shared__ f32 part[2][ROW_THREADS / 32][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  constexpr int W = ROW_THREADS / 32;
+  const i64 j = (i64)blockIdx.x * 32 + lane;
+  f32 sg = 0.0f, sb = 0.0f;
+  if (j < p.n) {
+    const f32* q = reinterpret_cast<const f32*>(p.partial) + j;
+#pragma unroll 4
+    for (i64 l = warp; l < p.lines; l += W) {
+      sg += q[l * 2 * p.n];
+      sb += q[l * 2 * p.n + p.n];
+    }
+  }
+  part[0][warp][lane] = sg;
+  part[1][warp][lane] = sb;
+  __syncthreads();
+  if (warp < 2 && j < p.n) {
+    f32 s = 0.0f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) s += part[warp][w][lane];
+    row_narrow(s, reinterpret_cast<param_t*>(warp == 0 ? p.dgamma : p.dbeta)[j]);
+  }
+}
+#elif NORM_COLS
+// Sums over `chunk` rows of 32 columns per CTA (rows too long for acc_rows_norm_grad's registers).
+extern "C" __global__ void __launch_bounds__(ROW_THREADS) acc_rows_norm_cols(const __grid_constant__ Params p) {
+  __shared__ f32 part[2][ROW_THREADS / 32][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  constexpr int W = ROW_THREADS / 32;
+  const i64 cols = (p.n + 31) / 32;
+  const i64 j = (blockIdx.x % cols) * 32 + lane, line = blockIdx.x / cols;
+  const i64 r1 = (line + 1) * p.chunk < p.rows ? (line + 1) * p.chunk : p.rows;
+  f32 sg = 0.0f, sb = 0.0f;
+  if (j < p.n)
+#pragma unroll 4
+    for (i64 r = line * p.chunk + warp; r < r1; r += W) {
+      const f32 d = row_wide(reinterpret_cast<const row_t*>(p.dy)[r * p.n + j]);
+      const f32 xh = (row_wide(reinterpret_cast<const row_t*>(p.x)[r * p.n + j]) - reinterpret_cast<const f32*>(p.mean)[r]) *
+                     reinterpret_cast<const f32*>(p.rstd)[r];
+      sg = fmaf(d, xh, sg);
+      sb += d;
+    }
+  part[0][warp][lane] = sg;
+  part[1][warp][lane] = sb;
+  __syncthreads();
+  if (warp < 2 && j < p.n) {
+    f32 s = 0.0f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) s += part[warp][w][lane];
+    reinterpret_cast<f32*>(p.partial)[line * 2 * p.n + warp * p.n + j] = s;
+  }
+}
+#else
+extern "C" __global__ void __launch_bounds__(ROW_THREADS) acc_rows_norm_grad(const __grid_constant__ Params p) {
+#if NORM_WARPS > 1
+  __shared__ f32 red[2][ROW_THREADS / 32][2];
+#else
+  f32(*red)[ROW_THREADS / 32][2] = nullptr;
+#endif
+  const int g = threadIdx.x % NORM_GROUP, sub = threadIdx.x / NORM_GROUP;
+  const int n = (int)p.n;
+  const f32 len = (f32)p.n;
+  constexpr int STEP = NORM_GROUP * NORM_VE;
+  const param_t* gamma = reinterpret_cast<const param_t*>(p.gamma);
+#if NORM_LONG
+  for (i64 row = blockIdx.x; row < p.rows; row += gridDim.x) {
+    const row_t* x = reinterpret_cast<const row_t*>(p.x) + row * p.n;
+    const row_t* dy = reinterpret_cast<const row_t*>(p.dy) + row * p.n;
+    row_t* dx = reinterpret_cast<row_t*>(p.dx) + row * p.n;
+    const f32 mean = reinterpret_cast<const f32*>(p.mean)[row], rstd = reinterpret_cast<const f32*>(p.rstd)[row];
+    f32 s[2] = {0.0f, 0.0f};
+    for (int j = g * NORM_VE; j < n; j += STEP) {
+      f32 v[NORM_VE], d[NORM_VE], ga[NORM_VE];
+      norm_wide(norm_load(x + j), v);
+      norm_wide(norm_load(dy + j), d);
+      norm_params(gamma + j, ga);
+#pragma unroll
+      for (int e = 0; e < NORM_VE; ++e) {
+        const f32 a = d[e] * ga[e];
+        s[0] += a;
+        s[1] = fmaf(a, (v[e] - mean) * rstd, s[1]);
+      }
+    }
+    norm_sum(s, red, 0);
+    const f32 ma = s[0] / len, mb = s[1] / len;
+    for (int j = g * NORM_VE; j < n; j += STEP) {
+      f32 v[NORM_VE], d[NORM_VE], ga[NORM_VE];
+      norm_wide(norm_load(x + j), v);
+      norm_wide(norm_load(dy + j), d);
+      norm_params(gamma + j, ga);
+#pragma unroll
+      for (int e = 0; e < NORM_VE; ++e) v[e] = rstd * (fmaf(-((v[e] - mean) * rstd), mb, fmaf(d[e], ga[e], -ma)));
+      norm_store(dx + j, v);
+    }
+    __syncthreads();                     // the next row writes the same slot
+  }
+#else
+  f32 sg[NORM_U * NORM_VE], sb[NORM_U * NORM_VE];
+#pragma unroll
+  for (int i = 0; i < NORM_U * NORM_VE; ++i) sg[i] = sb[i] = 0.0f;
+  norm_x bx[NORM_U], bd[NORM_U];
+  i64 row = (i64)blockIdx.x * NORM_ROWS + sub;
+  const i64 stride = (i64)gridDim.x * NORM_ROWS;
+  f32 mean = 0.0f, rstd = 0.0f;
+  int slot = 0;
+  // (a CTA's groups make the same number of trips: they share the barriers)
+  for (i64 first = (i64)blockIdx.x * NORM_ROWS; first < p.rows; first += stride, row += stride) {
+    const bool there = row < p.rows;
+    if (there) {
+      const row_t* x = reinterpret_cast<const row_t*>(p.x) + row * p.n;
+      const row_t* dy = reinterpret_cast<const row_t*>(p.dy) + row * p.n;
+#pragma unroll
+      for (int u = 0; u < NORM_U; ++u) {
+        const int j = u * STEP + g * NORM_VE;
+        if (j < n) {
+          bx[u] = norm_load(x + j);
+          bd[u] = norm_load(dy + j);
+        }
+      }
+      mean = reinterpret_cast<const f32*>(p.mean)[row];
+      rstd = reinterpret_cast<const f32*>(p.rstd)[row];
+    }
+    f32 s[2] = {0.0f, 0.0f};
+    if (there) {
+#pragma unroll
+      for (int u = 0; u < NORM_U; ++u) {
+        const int j = u * STEP + g * NORM_VE;
+        if (j < n) {
+          f32 v[NORM_VE], d[NORM_VE], ga[NORM_VE];
+          norm_wide(bx[u], v);
+          norm_wide(bd[u], d);
+          norm_params(gamma + j, ga);
+#pragma unroll
+          for (int e = 0; e < NORM_VE; ++e) {
+            const f32 xh = (v[e] - mean) * rstd, a = d[e] * ga[e];
+            s[0] += a;
+            s[1] = fmaf(a, xh, s[1]);
+            sg[u * NORM_VE + e] = fmaf(d[e], xh, sg[u * NORM_VE + e]);
+            sb[u * NORM_VE + e] += d[e];
+          }
+        }
+      }
+    }
+    norm_sum(s, red, slot);
+    slot ^= 1;
+    const f32 ma = s[0] / len, mb = s[1] / len;
+    if (there) {
+      row_t* dx = reinterpret_cast<row_t*>(p.dx) + row * p.n;
+#pragma unroll
+      for (int u = 0; u < NORM_U; ++u) {
+        const int j = u * STEP + g * NORM_VE;
+        if (j < n) {
+          f32 v[NORM_VE], d[NORM_VE], ga[NORM_VE];
+          norm_wide(bx[u], v);
+          norm_wide(bd[u], d);
+          norm_params(gamma + j, ga);
+#pragma unroll
+          for (int e = 0; e < NORM_VE; ++e) v[e] = rstd * (fmaf(-((v[e] - mean) * rstd), mb, fmaf(d[e], ga[e], -ma)));
+          norm_store(dx + j, v);
+        }
+      }
+    }
+  }
+  // this CTA's line: the groups' sums one after the other
+  f32* line = reinterpret_cast<f32*>(p.partial) + (i64)blockIdx.x * 2 * p.n;
+#if NORM_ROWS > 1
+  extern __shared__ f32 sums[];          // 2 n Floats
+#pragma unroll 1
+  for (int q = 0; q < NORM_ROWS; ++q) {
+    if (q == sub) {
+#pragma unroll
+      for (int u = 0; u < NORM_U; ++u)
+#pragma unroll
+        for (int e = 0; e < NORM_VE; ++e) {
+          const int j = u * STEP + g * NORM_VE + e;
+          if (j < n) {
+            sums[j] = q == 0 ? sg[u * NORM_VE + e] : sums[j] + sg[u * NORM_VE + e];
+            sums[n + j] = q == 0 ? sb[u * NORM_VE + e] : sums[n + j] + sb[u * NORM_VE + e];
+          }
+        }
+    }
+    __syncthreads();
+  }
+  for (int j = threadIdx.x; j < 2 * n; j += ROW_THREADS) line[j] = sums[j];
+#else
+#pragma unroll
+  for (int u = 0; u < NORM_U; ++u)
+#pragma unroll
+    for (int e = 0; e < NORM_VE; ++e) {
+      const int j = u * STEP + g * NORM_VE + e;
+      if (j < n) {
+        line[j] = sg[u * NORM_VE + e];
+        line[n + j] = sb[u * NORM_VE + e];
+      }
+    }
+#endif
+#endif
+}
+#endif

@@ -1,0 +1,484 @@
+// Statistics of a row of logits in one pass over it: the normaliser ln sum e^(x/tau), and behind it either
+//   log probabilities (ROW_DISTILL 0): the given token's log probability, the entropy, and the ROW_TOPK
+//     k largest logits with their indices; or
+//   a distillation loss (ROW_DISTILL 1): tau^2 sum q (ln q - ln p) against a teacher's few entries.
+//
+// Mathematics.  With c = log2(e)/tau and m the running maximum, every thread keeps Z = sum 2^t and
+// W = sum 2^t t over its elements, t = c (x - m), and moves both to a new maximum m' by Z' = s Z,
+// W' = s (W + d Z), d = c (m - m'), s = 2^d.  Threads, warps and CTAs join by the same rule.  Then
+//   lse = m/tau + ln Z,     entropy = ln Z - ln 2 W / Z.
+// Half: t = c x - M with M = c m rounded, one instruction; what the rounding shifts is known exactly and comes
+// off the end (M - c m).  Float: the subtraction first, since c m can leave the range (rows masked with the
+// type's lowest value); a Float element has twice the bytes to pay for the second instruction.
+// Sums are Float; products with 2^t = 0 are 0, so masked (-inf) elements count for nothing.
+//
+// A cluster of ROW_C CTAs shares a row (ROW_C > 1 when there are few rows) and joins through distributed
+// shared memory: no scratch in global memory, nothing that two launches could share.
+
+//   x, tok or ids: arrays; the outputs; n = row length; k = alternatives, or teacher entries per row
+struct Params { i64 x, tok, teacher, out0, out1, out2, out3, out4, rows, n, k, tau, err; };
+
+constexpr int ST_TILE = ROW_THREADS * ROW_U;     // blocks per tile
+constexpr int ST_WARPS = ROW_THREADS / 32;
+constexpr int ST_CAP = 2048;                     // candidate keys held in shared memory
+
+struct row_stat { f32 m, z, w; };
+struct st_shared {
+#if ROW_TOPK
+  u64 cand[ST_CAP];
+  int count;           // candidates, while they are being appended
+  int kept;            // candidates of this CTA at the end (read by the cluster's first CTA)
+  u64 key[ST_WARPS];
+#endif
+  row_stat part[ST_WARPS];
+  row_stat cta;
+  int warp_count[ST_WARPS];
+};
+
+// (a maximum of -inf, "nothing yet", stands at 0: its sums are 0)
+__device__ __forceinline__ f32 st_base(f32 m) { return m == -ROW_INF ? 0.0f : m; }
+__device__ __forceinline__ f32 st_shift(f32 from, f32 to, f32 c) {
+  if (from == -ROW_INF) return 0.0f;
+#if ROW_F16
+  return from * c - to * c;            // both rounded, as the elements saw them (--fmad=false)
+#else
+  return (from - to) * c;
+#endif
+}
+__device__ __forceinline__ row_stat st_join(const row_stat& a, const row_stat& b, f32 c) {
+  row_stat r;
+  r.m = fmaxf(a.m, b.m);
+  const f32 da = st_shift(a.m, r.m, c), db = st_shift(b.m, r.m, c);
+  const f32 sa = row_ex2(da), sb = row_ex2(db);
+  r.z = sa * a.z + sb * b.z;
+  // (d z is 0 times infinity when the other maximum is out of reach: that part is then 0)
+  r.w = (sa == 0.0f ? 0.0f : sa * fmaf(da, a.z, a.w)) + (sb == 0.0f ? 0.0f : sb * fmaf(db, b.z, b.w));
+  return r;
+}
+
+#if ROW_TOPK
+// Order of the alternatives in one whole number: the value (NaN above +inf, -0 equal to 0) in the upper 32 bits,
+// the complement of the index below it.  Larger is better, no two elements of a row are equal.
+__device__ __forceinline__ u32 st_order(f32 v) {
+  if (v != v) return 0xffffffffu;
+  const u32 u = __float_as_uint(v + 0.0f);
+  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+__device__ __forceinline__ f32 st_value(u32 o) {
+  if (o == 0xffffffffu) return ROW_NAN;
+  return __uint_as_float((o & 0x80000000u) ? (o & 0x7fffffffu) : ~o);
+}
+__device__ __forceinline__ u64 st_key(f32 v, int j) { return ((u64)st_order(v) << 32) | (u32)~j; }
+__device__ __forceinline__ int st_index(u64 key) { return (int)~(u32)key; }
+#define ST_NONE ((u64)0x007fffffffffffffull)     /* the best key of a -inf element: candidates lie above it */
+
+// The best k of the n candidates, in falling order, to the front of the list; returns how many there are.
+// Up to one candidate per thread: each counts the candidates above its own.  More (only rows in an unusual
+// order, or lists of many CTAs): a bitonic sort.
+__device__ __forceinline__ int st_compact(st_shared& sh, int n, int k) {
+  const int tid = threadIdx.x;
+  if (n <= ROW_THREADS) {
+    u64 key = 0;
+    int rank = 0;
+    if ((tid & ~31) < n) {
+      key = tid < n ? sh.cand[tid] : 0;
+      for (int i = 0; i < n; ++i) rank += sh.cand[i] > key ? 1 : 0;
+    }
+    __syncthreads();
+    if (tid < n && rank < k) sh.cand[rank] = key;
+    __syncthreads();
+  } else {
+    int size = ROW_THREADS;
+    while (size < n) size <<= 1;
+    for (int i = n + tid; i < size; i += ROW_THREADS) sh.cand[i] = 0;
+    __syncthreads();
+    for (int len = 2; len <= size; len <<= 1)
+      for (int d = len >> 1; d > 0; d >>= 1) {
+        for (int i = tid; i < size / 2; i += ROW_THREADS) {
+          const int lo = 2 * i - (i & (d - 1)), hi = lo + d;
+          const u64 a = sh.cand[lo], b = sh.cand[hi];
+          const bool falling = (lo & len) == 0;
+          if (falling ? a < b : a > b) { sh.cand[lo] = b; sh.cand[hi] = a; }
+        }
+        __syncthreads();
+      }
+  }
+  return n < k ? n : k;
+}
+#endif
+
+__device__ __forceinline__ u32 st_cluster_addr(const void* p, int rank) {
+  u32 a, r;
+  asm("{ .reg .u64 t; cvta.to.shared.u64 t, %1; cvt.u32.u64 %0, t; }" : "=r"(a) : "l"(p));
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void st_cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+extern "C" __global__ void __launch_bounds__(ROW_THREADS, ROW_MIN_BLOCKS)
+#if ROW_C > 1
+__cluster_dims__(ROW_C, 1, 1)
+#endif
+acc_rows_stats(const __grid_constant__ Params p) {
+  __shared__ st_shared sh;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const i64 row = blockIdx.x / ROW_C;
+  const int part = (int)(blockIdx.x % ROW_C);
+  const int n = (int)p.n, k = (int)p.k;
+  const row_span span(reinterpret_cast<const row_t*>(p.x) + row * p.n, n);
+  const int per = (span.blocks + ROW_C - 1) / ROW_C;
+  const int b0 = min(part * per, span.blocks), b1 = min(b0 + per, span.blocks);
+  const f32 tau = __uint_as_float((u32)p.tau);
+  const f32 c = ROW_LOG2E / tau;
+
+  row_stat st = {-ROW_INF, 0.0f, 0.0f};
+#if ROW_TOPK
+  int held = 0;                         // candidates in the list (the same in every thread)
+  u64 thr_key = ST_NONE;                // only elements above this key are candidates
+  f32 thr = -ROW_INF;                   // its value: a quick test for a whole chunk
+  if (tid == 0) sh.count = 0;
+#endif
+
+  uint4 cur[ROW_U], nxt[ROW_U];
+  const uint4 pad = make_uint4(ROW_PAD, ROW_PAD, ROW_PAD, ROW_PAD);
+#pragma unroll
+  for (int u = 0; u < ROW_U; ++u) {
+    const int i = b0 + u * ROW_THREADS + tid;
+    nxt[u] = i < b1 ? span.load(i) : pad;
+  }
+  for (int t = b0; t < b1; t += ST_TILE) {
+#pragma unroll
+    for (int u = 0; u < ROW_U; ++u) cur[u] = nxt[u];
+    if (t + ST_TILE < b1) {
+#pragma unroll
+      for (int u = 0; u < ROW_U; ++u) {
+        const int i = t + ST_TILE + u * ROW_THREADS + tid;
+        nxt[u] = i < b1 ? span.load(i) : pad;
+      }
+    }
+    // maxima: of each block and of the chunk (a NaN stays visible)
+    f32 mc;
+#if ROW_F16
+    u32 mb[ROW_U], mp;
+#pragma unroll
+    for (int u = 0; u < ROW_U; ++u) {
+      mb[u] = row_max_nan2(row_max_nan2(cur[u].x, cur[u].y), row_max_nan2(cur[u].z, cur[u].w));
+      mp = u == 0 ? mb[0] : row_max_nan2(mp, mb[u]);
+    }
+    {
+      f32 lo, hi;
+      row_h2x2(mp, lo, hi);
+      mc = row_max_nan(lo, hi);
+    }
+#else
+    f32 mb[ROW_U];
+#pragma unroll
+    for (int u = 0; u < ROW_U; ++u) {
+      f32 v[ROW_E];
+      row_unpack(cur[u], v);
+      mb[u] = row_max_nan(row_max_nan(v[0], v[1]), row_max_nan(v[2], v[3]));
+      mc = u == 0 ? mb[0] : row_max_nan(mc, mb[u]);
+    }
+#endif
+    // statistics
+    const f32 mn = fmaxf(st.m, mc);
+    if (mn > st.m) {
+      if (st.m != -ROW_INF) {
+        const f32 d = st_shift(st.m, mn, c), s = row_ex2(d);
+        st.w = s == 0.0f ? 0.0f : s * fmaf(d, st.z, st.w);
+        st.z *= s;
+      }
+      st.m = mn;
+    }
+#if ROW_F16
+    const f32 neg = -(st_base(st.m) * c);
+#define ST_T(x) fmaf(x, c, neg)
+#else
+    const f32 base = st_base(st.m);
+#define ST_T(x) (((x) - base) * c)
+#endif
+    f32 z0 = 0.0f, z1 = 0.0f, w0 = 0.0f, w1 = 0.0f;
+#pragma unroll
+    for (int u = 0; u < ROW_U; ++u) {
+      f32 v[ROW_E];
+      row_unpack(cur[u], v);
+#pragma unroll
+      for (int e = 0; e < ROW_E; e += 2) {
+        const f32 ta = ST_T(v[e]), tb = ST_T(v[e + 1]);
+        const f32 ea = row_ex2(ta), eb = row_ex2(tb);
+        z0 += ea;
+        z1 += eb;
+#if !ROW_DISTILL
+        // (a masked element has t = -inf and 2^t = 0: the bound keeps their product at 0)
+        w0 = fmaf(ea, fmaxf(ta, -1000.0f), w0);
+        w1 = fmaf(eb, fmaxf(tb, -1000.0f), w1);
+#endif
+      }
+    }
+    st.z += z0 + z1;
+    st.w += w0 + w1;
+
+#if ROW_TOPK
+    if (t == b0) {
+      // The first tile sets the threshold: with T the largest 16-bit prefix that k threads' maxima reach, the
+      // least key among k of those maxima.  k elements of the tile are at least that, few more pass it.
+      const u32 pre = mc == -ROW_INF ? 0u : (st_order(mc) >> 16);
+      u32 T = 0;
+      for (int bit = 15; bit >= 0; --bit) {
+        const u32 trial = T | (1u << bit);
+        if (__syncthreads_count(pre >= trial) >= k) T = trial;
+      }
+      if (T != 0) {
+        const int above = __syncthreads_count(pre > T);
+        const bool tie = pre == T;
+        const u32 ties = __ballot_sync(ACC_FULL_MASK, tie);
+        if (lane == 0) sh.warp_count[warp] = __popc(ties);
+        __syncthreads();
+        int before = __popc(ties & ((1u << lane) - 1));
+        for (int w = 0; w < warp; ++w) before += sh.warp_count[w];
+        u64 mine = ~(u64)0;
+        if (tie && before < k - above) {
+          u64 best = 0;
+#pragma unroll
+          for (int u = 0; u < ROW_U; ++u) {
+            f32 v[ROW_E];
+            row_unpack(cur[u], v);
+            const int j = span.first(t + u * ROW_THREADS + tid);
+#pragma unroll
+            for (int e = 0; e < ROW_E; ++e) {
+              const u64 key = st_key(v[e], j + e);
+              best = key > best ? key : best;
+            }
+          }
+          mine = best;
+        }
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) {
+          const u64 o = __shfl_xor_sync(ACC_FULL_MASK, mine, d);
+          mine = o < mine ? o : mine;
+        }
+        if (lane == 0) sh.key[warp] = mine;
+        __syncthreads();
+        for (int w = 0; w < ST_WARPS; ++w) mine = sh.key[w] < mine ? sh.key[w] : mine;
+        if (mine - 1 > thr_key) thr_key = mine - 1;
+      }
+    }
+    const bool hot = t == b0 ? mc != -ROW_INF : !(mc <= thr);
+    if (__syncthreads_or(hot)) {
+      if (hot) {
+#pragma unroll
+        for (int u = 0; u < ROW_U; ++u) {
+#if ROW_F16
+          f32 lo, hi;
+          row_h2x2(mb[u], lo, hi);
+          const f32 bm = row_max_nan(lo, hi);
+#else
+          const f32 bm = mb[u];
+#endif
+          const int j = span.first(t + u * ROW_THREADS + tid);
+          if (t == b0 ? st_order(bm) >= (u32)(thr_key >> 32) : !(bm <= thr)) {
+            f32 v[ROW_E];
+            row_unpack(cur[u], v);
+#pragma unroll
+            for (int e = 0; e < ROW_E; ++e) {
+              const u64 key = st_key(v[e], j + e);
+              if (key > thr_key) {
+                const int slot = atomicAdd(&sh.count, 1);
+                if (slot < ST_CAP) sh.cand[slot] = key;
+              }
+            }
+          }
+        }
+      }
+      __syncthreads();
+      int total = sh.count;
+      if (total > ST_CAP) {
+        // More candidates than the list holds (a row in rising order): take the tile in pieces of four elements per
+        // thread, and keep the best k of the list after each.
+        __syncthreads();
+        for (int q = 0; q < ROW_U * (ROW_E / 4); ++q) {
+          held = st_compact(sh, held, k);
+          if (held == k) thr_key = sh.cand[k - 1];
+          if (tid == 0) sh.count = held;
+          __syncthreads();
+#pragma unroll
+          for (int u = 0; u < ROW_U; ++u) {
+            f32 v[ROW_E];
+            row_unpack(cur[u], v);
+            const int j = span.first(t + u * ROW_THREADS + tid);
+#pragma unroll
+            for (int e = 0; e < ROW_E; ++e) {
+              if (u * (ROW_E / 4) + e / 4 == q) {
+                const u64 key = st_key(v[e], j + e);
+                if (key > thr_key) sh.cand[atomicAdd(&sh.count, 1)] = key;
+              }
+            }
+          }
+          __syncthreads();
+          held = sh.count;
+          __syncthreads();
+        }
+        total = held;
+      }
+      held = total;
+      if (t == b0 || held > k + 64) {
+        held = st_compact(sh, held, k);
+        if (held == k) {
+          thr_key = sh.cand[k - 1];
+          const f32 v = st_value((u32)(thr_key >> 32));
+          thr = v != v ? ROW_INF : v;
+        } else {
+          thr_key = ST_NONE;
+        }
+        if (tid == 0) sh.count = held;     // (read again only behind the next tile's barriers)
+      }
+    }
+#endif
+  }
+#if ROW_TOPK
+  held = st_compact(sh, held, k);
+  if (tid == 0) sh.kept = held;
+#endif
+  // join the statistics: lanes, warps, CTAs of the cluster
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) {
+    row_stat o;
+    o.m = __shfl_xor_sync(ACC_FULL_MASK, st.m, d);
+    o.z = __shfl_xor_sync(ACC_FULL_MASK, st.z, d);
+    o.w = __shfl_xor_sync(ACC_FULL_MASK, st.w, d);
+    st = st_join(st, o, c);
+  }
+  if (lane == 0) sh.part[warp] = st;
+  __syncthreads();
+  st = sh.part[0];
+#pragma unroll
+  for (int w = 1; w < ST_WARPS; ++w) st = st_join(st, sh.part[w], c);
+#if ROW_C > 1
+  if (tid == 0) sh.cta = st;
+  st_cluster_sync();
+  if (part == 0) {
+    for (int r = 1; r < ROW_C; ++r) {
+      const u32 a = st_cluster_addr(&sh.cta, r);
+      row_stat o;
+      asm volatile("ld.shared::cluster.f32 %0, [%3];\n ld.shared::cluster.f32 %1, [%3 + 4];\n ld.shared::cluster.f32 %2, [%3 + 8];"
+                   : "=f"(o.m), "=f"(o.z), "=f"(o.w) : "r"(a));
+      st = st_join(st, o, c);
+    }
+#if ROW_TOPK
+    for (int r = 1; r < ROW_C; ++r) {
+      int more;
+      asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(more) : "r"(st_cluster_addr(&sh.kept, r)));
+      if (tid < more) {                  // (at most k <= 128 of them: one per thread)
+        u64 key;
+        asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(key) : "r"(st_cluster_addr(&sh.cand[tid], r)));
+        sh.cand[held + tid] = key;
+      }
+      held += more;
+    }
+    __syncthreads();
+    held = st_compact(sh, held, k);
+#endif
+  }
+  st_cluster_sync();                     // nobody leaves while its shared memory is being read
+  if (part != 0) return;
+#endif
+
+  // a row without an element above -inf has no distribution: its normaliser is -inf
+  f32 lse = -ROW_INF;
+  if (st.m != -ROW_INF || st.z != 0.0f) {
+    lse = st_base(st.m) / tau + logf(st.z);
+#if ROW_F16
+    const f32 base = st_base(st.m);
+    lse += ROW_LN2 * fmaf(-base, c, base * c);
+#endif
+  }
+#if ROW_DISTILL
+  // The teacher's entries, one warp: with e_i = exp((t_i - max t)/tau) and E their sum, q_i = e_i / E and
+  // loss = tau^2 (sum e_i ((t_i - max t) - s_i) / (tau E) - ln E + lse).
+  if (warp == 0) {
+    const i32* ids = reinterpret_cast<const i32*>(p.tok) + row * p.k;
+    const teacher_t* ts = reinterpret_cast<const teacher_t*>(p.teacher) + row * p.k;
+    f32 mt = -ROW_INF;
+    bool bad = false;
+    for (int i = lane; i < k; i += 32) {
+      const int id = ids[i];
+      bad = bad || id >= n;
+      if (id >= 0 && id < n) mt = row_max_nan(mt, row_wide(ts[i]));
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) mt = row_max_nan(mt, __shfl_xor_sync(ACC_FULL_MASK, mt, d));
+    f32 es = 0.0f, as = 0.0f;
+    for (int i = lane; i < k; i += 32) {
+      const int id = ids[i];
+      if (id >= 0 && id < n) {
+        const f32 dt = mt == -ROW_INF ? -ROW_INF : row_wide(ts[i]) - mt;
+        const f32 e = row_ex2(dt * c);
+        if (e != 0.0f) {
+          es += e;
+          as += e * ((dt - row_wide(span.x[id])) / tau);
+        }
+      }
+    }
+    es = row_warp_sum(es);
+    as = row_warp_sum(as);
+    bad = __any_sync(ACC_FULL_MASK, bad);
+    if (lane == 0) {
+      f32 loss = 0.0f;                   // no entry, no loss
+      if (es != 0.0f) loss = lse == -ROW_INF ? ROW_INF : tau * tau * (as / es - logf(es) + lse);
+      if (bad) {
+        acc_fail(p.err, 1003);           // "index out of bounds", reported by the next download or b200_sync
+        loss = ROW_NAN;
+      }
+      reinterpret_cast<f32*>(p.out0)[row] = loss;
+      reinterpret_cast<f32*>(p.out1)[row] = lse;
+    }
+  }
+#else
+  if (tid == 0) {
+    const i64 tok = (i64) reinterpret_cast<const token_t*>(p.tok)[row];
+    f32 logp = 0.0f;                     // no given token
+    if (tok >= n) {
+      acc_fail(p.err, 1003);
+      logp = ROW_NAN;
+    } else if (tok >= 0) {
+      logp = lse == -ROW_INF ? -ROW_INF : row_wide(span.x[tok]) - lse;
+    }
+    reinterpret_cast<f32*>(p.out0)[row] = logp;
+    reinterpret_cast<f32*>(p.out1)[row] = lse;
+    reinterpret_cast<f32*>(p.out2)[row] = lse == -ROW_INF ? 0.0f : logf(st.z) - ROW_LN2 * (st.w / st.z);
+  }
+#if ROW_TOPK
+  __syncthreads();
+  if (held < k) {
+    // All elements above -inf are in the list.  The places behind them go to -inf elements, lowest index first: they
+    // are among the row's first 2k - 1 (at most 255) elements.
+    bool free_one = tid < n && tid < 2 * k;
+    for (int i = 0; i < held; ++i) free_one = free_one && st_index(sh.cand[i]) != tid;
+    const u32 ones = __ballot_sync(ACC_FULL_MASK, free_one);
+    if (lane == 0) sh.warp_count[warp] = __popc(ones);
+    __syncthreads();
+    int at = held + __popc(ones & ((1u << lane) - 1)), all = held;
+    for (int w = 0; w < ST_WARPS; ++w) {
+      if (w < warp) at += sh.warp_count[w];
+      all += sh.warp_count[w];
+    }
+    if (free_one && at < k) sh.cand[at] = st_key(-ROW_INF, tid);
+    held = all < k ? all : k;
+    __syncthreads();
+  }
+  if (tid < k) {
+    int id = -1;                         // a row shorter than k ends in (-1, -inf)
+    f32 logp = -ROW_INF;
+    if (tid < held) {
+      const u64 key = sh.cand[tid];
+      id = st_index(key);
+      if (lse != -ROW_INF) logp = st_value((u32)(key >> 32)) - lse;
+    }
+    reinterpret_cast<i32*>(p.out3)[row * p.k + tid] = id;
+    reinterpret_cast<f32*>(p.out4)[row * p.k + tid] = logp;
+  }
+#endif
+#endif
+}

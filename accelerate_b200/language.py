@@ -1278,7 +1278,7 @@ def apply(f, *args):
 def aforeign(name, fallback, *args):
     """``Aforeign`` (AST.hs; Interpreter.hs:217): a backend that has no foreign implementation under ``name``
     runs the pure Accelerate function given as the fallback, which is what the interpreter always does and
-    what this backend does."""
+    what this backend does for functions of other backends.  (Its own foreign functions: ``rows``.)"""
     del name
     return apply(fallback, *args)
 
@@ -1303,7 +1303,7 @@ def pipe(f, g):
 
 
 def _is_control(n):
-    return n.kind in ("acond", "awhile", "apply")
+    return n.kind in ("acond", "awhile", "apply", "aforeign")
 
 
 def _reach(roots, stop=()):
@@ -1391,7 +1391,8 @@ class _Emitter:
                     for n in _reach([r.node for r in res]):
                         if skip(n) or id(n) in here:
                             continue
-                        free = c.kind != "acond" and not _depends_on(n, [q.node for q in params], memo)
+                        # (the definition behind a foreign function stays inside it: it may never run)
+                        free = c.kind not in ("acond", "aforeign") and not _depends_on(n, [q.node for q in params], memo)
                         count[id(n)] = count.get(id(n), 0) + 1
                         if free or count[id(n)] > 1:
                             hoisted.setdefault(id(c), []).append(n)
@@ -1414,6 +1415,9 @@ class _Emitter:
                 args = "(args " + " ".join(a.name for a in n.args) + ")"
                 if n.kind == "acond":
                     text = f"(acond {n.pred.sx}\n" + "\n".join(parts) + ")"
+                elif n.kind == "aforeign":
+                    name, consts = n.foreign
+                    text = f"(aforeign {name} (consts{''.join(' ' + c for c in consts)})\n" + "\n".join(parts) + f"\n{pad}    {args})"
                 else:
                     text = f"({n.kind}\n" + "\n".join(parts) + f"\n{pad}    {args})"
                 lines.append(f"{pad}(let {lhs} {text})")

@@ -1119,6 +1119,10 @@ void parse_node(Program& p, std::vector<Node>& into, const Sx& bind, Scope& sc) 
   } else if (k == "apply") {
     n.body.push_back(parse_body(p, x[1], sc, true));
     for (size_t j = 1; j < x[2].size(); ++j) n.args.push_back(sc.array(x[2].k[j].s));
+  } else if (k == "aforeign") {
+    // (aforeign NAME (consts c..) (afun ..) (args a..)): the interpreter applies the pure function (Interp:217)
+    n.body.push_back(parse_body(p, x[3], sc, true));
+    for (size_t j = 1; j < x[4].size(); ++j) n.args.push_back(sc.array(x[4].k[j].s));
   } else if (k == "atrace") {
     // (atrace (hex MESSAGE) (show a..) (args b..))
     const std::string digits = x[1].size() > 1 ? x[1].k[1].s : std::string();
@@ -1254,8 +1258,8 @@ void run_node(Program& p, const Node& n, Env& env) {
       st = call_body(p, n.body[1], st, env);
     }
     for (size_t i = 0; i < n.outs.size(); ++i) vals[n.outs[i]] = st[i];
-  } else if (k == "apply") {
-    // Interp:215
+  } else if (k == "apply" || k == "aforeign") {
+    // Interp:215, 217
     std::vector<ArrayP> as;
     for (int a : n.args) as.push_back(vals[a]);
     std::vector<ArrayP> r = call_body(p, n.body[0], as, env);
