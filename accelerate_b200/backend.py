@@ -55,6 +55,8 @@ def lib():
         l.b200_array_shape.argtypes = [vp, ctypes.c_uint64, i64p]
         l.b200_array_num_leaves.argtypes = [vp, ctypes.c_uint64, ctypes.POINTER(ctypes.c_int)]
         l.b200_array_leaf_type.argtypes = [vp, ctypes.c_uint64, ctypes.c_int, ctypes.POINTER(cp)]
+        l.b200_array_info.argtypes = [vp, ctypes.c_uint64, ctypes.c_int, ctypes.POINTER(ctypes.c_int), i64p, ctypes.c_int,
+                                      ctypes.POINTER(ctypes.c_int), ctypes.POINTER(ctypes.c_int32)]
         l.b200_array_devptr.argtypes = [vp, ctypes.c_uint64, ctypes.c_int, ctypes.POINTER(vp)]
         l.b200_program_load.argtypes = [vp, cp, ctypes.c_size_t, ctypes.POINTER(vp)]
         l.b200_program_free.argtypes = [vp]
@@ -115,25 +117,49 @@ def kernel_source(text, node=0):
     return buf.value.decode()
 
 
-class DeviceArray:
-    """A device-resident array (struct-of-arrays) owned by a context."""
+_LEAVES, _ELT_TEXT = {}, {}
 
-    def __init__(self, ctx, ident, elt=None):
+
+def _leaf_types(elt):
+    """Scalar types of an element type's leaves (remembered: asked for with every array)."""
+    try:
+        r = _LEAVES.get(elt)
+        if r is None:
+            r = _LEAVES[elt] = L.flatten_ty(elt)
+        return r
+    except TypeError:                    # a list in the place of a tuple
+        return L.flatten_ty(elt)
+
+
+def _elt_text(elt):
+    try:
+        r = _ELT_TEXT.get(elt)
+        if r is None:
+            r = _ELT_TEXT[elt] = L.ty_sx(elt).encode()
+        return r
+    except TypeError:
+        return L.ty_sx(elt).encode()
+
+
+class DeviceArray:
+    """A device-resident array (struct-of-arrays) owned by a context.  Whoever made it and knows its element type and
+    shape passes both; otherwise the library is asked, once."""
+
+    def __init__(self, ctx, ident, elt=None, shape=None):
         self.ctx, self.id = ctx, ident
-        l = lib()
-        r = ctypes.c_int()
-        _check(l.b200_array_rank(ctx.h, ident, ctypes.byref(r)))
-        sh = (ctypes.c_int64 * max(1, r.value))()
-        _check(l.b200_array_shape(ctx.h, ident, sh))
-        self.shape = tuple(int(sh[i]) for i in range(r.value))
-        n = ctypes.c_int()
-        _check(l.b200_array_num_leaves(ctx.h, ident, ctypes.byref(n)))
-        self.leaf_types = []
-        for k in range(n.value):
-            s = ctypes.c_char_p()
-            _check(l.b200_array_leaf_type(ctx.h, ident, k, ctypes.byref(s)))
-            self.leaf_types.append(s.value.decode())
-        self.elt = elt if elt is not None else (self.leaf_types[0] if n.value == 1 else tuple(self.leaf_types))
+        if elt is not None and shape is not None:
+            self.elt, self.shape, self.leaf_types = elt, shape, _leaf_types(elt)
+            return
+        rank, leaves = ctypes.c_int(), ctypes.c_int()
+        for most_rank, most_leaves in ((8, 32), (1 << 10, 1 << 16)):
+            sh, types = (ctypes.c_int64 * most_rank)(), (ctypes.c_int32 * most_leaves)()
+            rc = lib().b200_array_info(ctx.h, ident, most_rank, ctypes.byref(rank), sh, most_leaves, ctypes.byref(leaves), types)
+            if rc == 0:
+                break
+        _check(rc)
+        self.shape = tuple(sh[:rank.value])
+        self.leaf_types = [L.SCALARS[k] for k in types[:leaves.value]]
+        self.elt = elt if elt is not None else (self.leaf_types[0] if leaves.value == 1 else tuple(self.leaf_types))
 
     def devptr(self, leaf=0):
         p = ctypes.c_void_p()
@@ -210,8 +236,8 @@ class Context:
     def array(self, elt, shape):
         ident = ctypes.c_uint64()
         sh = (ctypes.c_int64 * max(1, len(shape)))(*shape)
-        _check(lib().b200_array_new(self.h, L.ty_sx(elt).encode(), len(shape), sh, ctypes.byref(ident)))
-        return DeviceArray(self, ident.value, elt)
+        _check(lib().b200_array_new(self.h, _elt_text(elt), len(shape), sh, ctypes.byref(ident)))
+        return DeviceArray(self, ident.value, elt, tuple(map(int, shape)))
 
     def from_host(self, a, elt=None):
         """Upload an ndarray, or a tuple of equal-shape ndarrays (array of tuples)."""
@@ -256,8 +282,8 @@ class Context:
         ident = ctypes.c_uint64()
         sh = (ctypes.c_int64 * max(1, len(shape)))(*shape)
         arr = (ctypes.c_void_p * len(ptrs))(*ptrs)
-        _check(lib().b200_array_wrap(self.h, L.ty_sx(elt).encode(), len(shape), sh, arr, ctypes.byref(ident)))
-        return DeviceArray(self, ident.value, elt)
+        _check(lib().b200_array_wrap(self.h, _elt_text(elt), len(shape), sh, arr, ctypes.byref(ident)))
+        return DeviceArray(self, ident.value, elt, tuple(map(int, shape)))
 
     # programs ---------------------------------------------------------------
     def load(self, text):

@@ -374,6 +374,18 @@ int b200_array_leaf_type(b200_ctx* ctx, uint64_t id, int leaf, const char** name
   *name = ty_name[a->leaf_ty[leaf]];
   B200_END
 }
+int b200_array_info(b200_ctx* ctx, uint64_t id, int max_rank, int* rank, int64_t* shape, int max_leaves, int* leaves, int32_t* types) {
+  B200_TRY
+  if (!ctx || !rank || !leaves || max_rank < 0 || max_leaves < 0 || (max_rank && !shape) || (max_leaves && !types)) throw Error(B200_ERR_ARG, "bad argument");
+  std::lock_guard<std::mutex> g(ctx->c.mu);
+  DevArrayP a = lookup(ctx->c, id);
+  *rank = (int)a->shape.size();
+  *leaves = (int)a->leaf_ty.size();
+  if (*rank > max_rank || *leaves > max_leaves) throw Error(B200_ERR_ARG, "the array has more dimensions or leaves than there is room for");
+  for (int d = 0; d < *rank; ++d) shape[d] = a->shape[d];
+  for (int l = 0; l < *leaves; ++l) types[l] = (int32_t)a->leaf_ty[l];
+  B200_END
+}
 int b200_array_devptr(b200_ctx* ctx, uint64_t id, int leaf, void** ptr) {
   B200_TRY
   std::lock_guard<std::mutex> g(ctx->c.mu);

@@ -151,6 +151,7 @@ struct NormShape {
   Variant variant() const {
     return {{"ROW_THREADS", str(threads)}, {"NORM_VE", str(ve)}, {"NORM_WARPS", str(warps)}, {"NORM_U", str(u)}, {"NORM_LONG", whole ? "0" : "1"}};
   }
+  uint64_t key() const { return (uint64_t)ve << 40 | (uint64_t)warps << 32 | (uint64_t)u << 16 | (uint64_t)(threads / 32) << 8 | (whole ? 1 : 0); }
   int rows() const { return threads / 32 / warps; }
 };
 // the next size of the list 1 2 3 4 6 8 12 16 ...: few kernels for all lengths
@@ -216,6 +217,17 @@ uint64_t float_bits(double v) {
   memcpy(&b, &f, 4);
   return b;
 }
+// The kernel of a foreign node for a launch shape: `key` identifies the shape, `variant` spells it out, once.
+template <class V> CompiledKernel& shape_kernel(Ctx& c, NodeState& st, uint64_t key, const char* skeleton, V variant, const char* entry, int threads, size_t smem) {
+  auto it = st.shape_memo.find(key);
+  if (it != st.shape_memo.end()) {
+    c.mem_hits++;
+    return *it->second;
+  }
+  CompiledKernel& k = node_kernel(c, st, skeleton, variant(), entry, threads, smem);
+  st.shape_memo[key] = &k;
+  return k;
+}
 void launch(Ctx& c, CompiledKernel& k, int64_t grid, int threads, size_t smem, std::vector<uint64_t> params) {
   if (grid <= 0) return;
   if (grid > 2147483647LL) throw Error(B200_ERR_UNSUPPORTED, "grid too large");
@@ -258,7 +270,7 @@ void Program::exec_foreign(const Node& n, Env& env) {
       env[n.outs[1]] = top;
       if (rows == 0) break;
       const int ctas = ctas_per_row(rows, cols, elt_bytes, c.sm_count, 8);
-      CompiledKernel& ker = node_kernel(c, st, "rows_stats", stats_variant(ctas), "acc_rows_stats", kThreads, 0);
+      CompiledKernel& ker = shape_kernel(c, st, (uint64_t)ctas, "rows_stats", [&] { return stats_variant(ctas); }, "acc_rows_stats", kThreads, 0);
       launch(c, ker, rows * ctas, kThreads, 0,
              {ptr_of(x), ptr_of(*a[0]), 0, ptr_of(*stats, 0), ptr_of(*stats, 1), ptr_of(*stats, 2), ptr_of(*top, 0), ptr_of(*top, 1),
               (uint64_t)rows, (uint64_t)cols, (uint64_t)k, float_bits(1.0), err});
@@ -276,7 +288,7 @@ void Program::exec_foreign(const Node& n, Env& env) {
         env[n.outs[1]] = lse;
         if (rows == 0) break;
         const int ctas = ctas_per_row(rows, cols, elt_bytes, c.sm_count, 8);
-        CompiledKernel& ker = node_kernel(c, st, "rows_stats", stats_variant(ctas), "acc_rows_stats", kThreads, 0);
+        CompiledKernel& ker = shape_kernel(c, st, (uint64_t)ctas, "rows_stats", [&] { return stats_variant(ctas); }, "acc_rows_stats", kThreads, 0);
         launch(c, ker, rows * ctas, kThreads, 0,
                {ptr_of(x), ptr_of(*a[0]), ptr_of(*a[1]), ptr_of(*loss), ptr_of(*lse), 0, 0, 0, (uint64_t)rows, (uint64_t)cols, (uint64_t)k,
                 float_bits(n.consts[0]), err});
@@ -287,7 +299,7 @@ void Program::exec_foreign(const Node& n, Env& env) {
         env[n.outs[0]] = dx;
         if (rows == 0 || cols == 0) break;
         const int ctas = ctas_per_row(rows, cols, elt_bytes, c.sm_count, 16);
-        CompiledKernel& ker = node_kernel(c, st, "rows_distill_grad", distill_grad_variant(ctas), "acc_rows_distill_grad", kThreads, 0);
+        CompiledKernel& ker = shape_kernel(c, st, (uint64_t)ctas, "rows_distill_grad", [&] { return distill_grad_variant(ctas); }, "acc_rows_distill_grad", kThreads, 0);
         launch(c, ker, rows * ctas, kThreads, 0,
                {ptr_of(x), ptr_of(*a[0]), ptr_of(*a[1]), ptr_of(*a[3]), ptr_of(*a[4]), ptr_of(*dx), (uint64_t)rows, (uint64_t)cols, (uint64_t)k,
                 float_bits(n.consts[0]), err});
@@ -302,7 +314,7 @@ void Program::exec_foreign(const Node& n, Env& env) {
       if (rows == 0) break;
       const bool wide = x.aligned16() && y->aligned16() && a[0]->aligned16() && a[1]->aligned16() && cols * elt_bytes % 16 == 0;
       const NormShape s = norm_shape(cols, wide ? 16 / elt_bytes : 1, kNormElems, kNormWarps, rows, c.sm_count);
-      CompiledKernel& ker = node_kernel(c, st, "rows_norm", s.variant(), "acc_rows_norm", s.threads, 0);
+      CompiledKernel& ker = shape_kernel(c, st, s.key(), "rows_norm", [&] { return s.variant(); }, "acc_rows_norm", s.threads, 0);
       launch(c, ker, (rows + s.rows() - 1) / s.rows(), s.threads, 0,
              {ptr_of(x), ptr_of(*a[0]), ptr_of(*a[1]), ptr_of(*y), ptr_of(*stats, 0), ptr_of(*stats, 1), (uint64_t)rows, (uint64_t)cols, float_bits(n.consts[0])});
       break;
@@ -318,10 +330,17 @@ void Program::exec_foreign(const Node& n, Env& env) {
       if (cols == 0) break;
       const bool wide = x.aligned16() && dx->aligned16() && a[3]->aligned16() && a[0]->aligned16() && cols * elt_bytes % 16 == 0;
       const NormShape s = norm_shape(cols, wide ? 16 / elt_bytes : 1, kNormGradElems, kNormGradWarps, rows, c.sm_count);
-      Variant var = s.variant();
-      var["NORM_SUMS"] = var["NORM_COLS"] = "0";
+      // (one source for three kernels: which of them it compiles to)
+      auto which = [&](bool sums, bool cols_) {
+        return [&, sums, cols_] {
+          Variant v = sums || cols_ ? norm_shape(1, 1, 1, 1, 1, 1).variant() : s.variant();
+          v["NORM_SUMS"] = sums ? "1" : "0";
+          v["NORM_COLS"] = cols_ ? "1" : "0";
+          return v;
+        };
+      };
       const size_t smem = s.whole && s.rows() > 1 ? (size_t)cols * 8 : 0;
-      CompiledKernel& ker = node_kernel(c, st, "rows_norm_grad", var, "acc_rows_norm_grad", s.threads, smem);
+      CompiledKernel& ker = shape_kernel(c, st, s.key(), "rows_norm_grad", which(false, false), "acc_rows_norm_grad", s.threads, smem);
       const int64_t grid = std::min<int64_t>((rows + s.rows() - 1) / s.rows(), (int64_t)c.sm_count * ker.max_blocks_per_sm);
       // lines of partial sums: one per CTA; for long rows one per `chunk` rows
       const int64_t tiles = (cols + 31) / 32;
@@ -334,16 +353,11 @@ void Program::exec_foreign(const Node& n, Env& env) {
       const std::vector<uint64_t> params = {ptr_of(x), ptr_of(*a[0]), ptr_of(*a[2], 0), ptr_of(*a[2], 1), ptr_of(*a[3]), ptr_of(*dx),
                                             (uint64_t)(uintptr_t)partial->ptr, ptr_of(*dgamma), ptr_of(*dbeta), (uint64_t)rows, (uint64_t)cols, (uint64_t)lines, (uint64_t)chunk};
       launch(c, ker, grid, s.threads, smem, params);
-      Variant sums = norm_shape(1, 1, 1, 1, 1, 1).variant();
-      sums["NORM_SUMS"] = "0";
-      sums["NORM_COLS"] = "1";
       if (!s.whole) {
-        CompiledKernel& kc = node_kernel(c, st, "rows_norm_grad", sums, "acc_rows_norm_cols", kThreads, 0);
+        CompiledKernel& kc = shape_kernel(c, st, 1, "rows_norm_grad", which(false, true), "acc_rows_norm_cols", kThreads, 0);
         launch(c, kc, lines * tiles, kThreads, 0, params);
       }
-      sums["NORM_SUMS"] = "1";
-      sums["NORM_COLS"] = "0";
-      CompiledKernel& ks = node_kernel(c, st, "rows_norm_grad", sums, "acc_rows_norm_sums", kThreads, 0);
+      CompiledKernel& ks = shape_kernel(c, st, 2, "rows_norm_grad", which(true, false), "acc_rows_norm_sums", kThreads, 0);
       launch(c, ks, tiles, kThreads, 0, params);
       break;
     }

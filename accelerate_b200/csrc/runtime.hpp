@@ -147,6 +147,7 @@ struct Ctx {
 struct NodeState {
   Glue glue;
   bool has_glue = false;
+  std::map<uint64_t, CompiledKernel*> shape_memo;       // the same by a foreign node's launch shape (rows.cpp)
   std::map<std::string, CompiledKernel*> kernel_memo;   // by skeleton, entry point and variant (entries of Ctx::kernels, which only grows)
 };
 struct Program {

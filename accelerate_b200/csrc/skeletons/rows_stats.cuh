@@ -21,11 +21,15 @@ struct Params { i64 x, tok, teacher, out0, out1, out2, out3, out4, rows, n, k, t
 constexpr int ST_TILE = ROW_THREADS * ROW_U;     // blocks per tile
 constexpr int ST_WARPS = ROW_THREADS / 32;
 constexpr int ST_CAP = 2048;                     // candidate keys held in shared memory
+constexpr int ST_BATCH = ST_CAP / 2;             // elements looked at between two looks at the list
 
 struct row_stat { f32 m, z, w; };
 struct st_shared {
 #if ROW_TOPK
   u64 cand[ST_CAP];
+  uint4 hot[ST_TILE];  // blocks of the tile that may hold candidates,
+  int hot_block[ST_TILE];  // and their numbers
+  int hot_count[2];    // of this tile and the next
   int count;           // candidates, while they are being appended
   int kept;            // candidates of this CTA at the end (read by the cluster's first CTA)
   u64 key[ST_WARPS];
@@ -56,7 +60,6 @@ __device__ __forceinline__ row_stat st_join(const row_stat& a, const row_stat& b
   return r;
 }
 
-#if ROW_TOPK
 // Order of the alternatives in one whole number: the value (NaN above +inf, -0 equal to 0) in the upper 32 bits,
 // the complement of the index below it.  Larger is better, no two elements of a row are equal.
 __device__ __forceinline__ u32 st_order(f32 v) {
@@ -70,8 +73,14 @@ __device__ __forceinline__ f32 st_value(u32 o) {
 }
 __device__ __forceinline__ u64 st_key(f32 v, int j) { return ((u64)st_order(v) << 32) | (u32)~j; }
 __device__ __forceinline__ int st_index(u64 key) { return (int)~(u32)key; }
+#if ROW_F16
+__device__ __forceinline__ f32 st_block_max(u32 m) { f32 lo, hi; row_h2x2(m, lo, hi); return row_max_nan(lo, hi); }
+#else
+__device__ __forceinline__ f32 st_block_max(f32 m) { return m; }
+#endif
 #define ST_NONE ((u64)0x007fffffffffffffull)     /* the best key of a -inf element: candidates lie above it */
 
+#if ROW_TOPK
 // The best k of the n candidates, in falling order, to the front of the list; returns how many there are.
 // Up to one candidate per thread: each counts the candidates above its own.  More (only rows in an unusual
 // order, or lists of many CTAs): a bitonic sort.
@@ -138,7 +147,9 @@ acc_rows_stats(const __grid_constant__ Params p) {
   int held = 0;                         // candidates in the list (the same in every thread)
   u64 thr_key = ST_NONE;                // only elements above this key are candidates
   f32 thr = -ROW_INF;                   // its value: a quick test for a whole chunk
-  if (tid == 0) sh.count = 0;
+  int parity = 0;
+  if (tid == 0) sh.count = sh.hot_count[0] = sh.hot_count[1] = 0;
+  __syncthreads();
 #endif
 
   uint4 cur[ROW_U], nxt[ROW_U];
@@ -167,11 +178,7 @@ acc_rows_stats(const __grid_constant__ Params p) {
       mb[u] = row_max_nan2(row_max_nan2(cur[u].x, cur[u].y), row_max_nan2(cur[u].z, cur[u].w));
       mp = u == 0 ? mb[0] : row_max_nan2(mp, mb[u]);
     }
-    {
-      f32 lo, hi;
-      row_h2x2(mp, lo, hi);
-      mc = row_max_nan(lo, hi);
-    }
+    mc = st_block_max(mp);
 #else
     f32 mb[ROW_U];
 #pragma unroll
@@ -222,8 +229,9 @@ acc_rows_stats(const __grid_constant__ Params p) {
 
 #if ROW_TOPK
     if (t == b0) {
-      // The first tile sets the threshold: with T the largest 16-bit prefix that k threads' maxima reach, the
-      // least key among k of those maxima.  k elements of the tile are at least that, few more pass it.
+      // The first tile sets the threshold.  With T the largest 16-bit prefix that k threads' maxima reach, take all
+      // maxima above T and, thread by thread, as many at T as make k: the least key among them (each rounded down to
+      // the end of its block) is reached by k elements of the tile, and few more pass it.
       const u32 pre = mc == -ROW_INF ? 0u : (st_order(mc) >> 16);
       u32 T = 0;
       for (int bit = 15; bit >= 0; --bit) {
@@ -232,109 +240,68 @@ acc_rows_stats(const __grid_constant__ Params p) {
       }
       if (T != 0) {
         const int above = __syncthreads_count(pre > T);
-        const bool tie = pre == T;
-        const u32 ties = __ballot_sync(ACC_FULL_MASK, tie);
+        const u32 ties = __ballot_sync(ACC_FULL_MASK, pre == T);
         if (lane == 0) sh.warp_count[warp] = __popc(ties);
         __syncthreads();
         int before = __popc(ties & ((1u << lane) - 1));
         for (int w = 0; w < warp; ++w) before += sh.warp_count[w];
-        u64 mine = ~(u64)0;
-        if (tie && before < k - above) {
-          u64 best = 0;
+        u64 least = ~(u64)0;
+        if (pre == T && before < k - above) {
+          int last = 0;
 #pragma unroll
-          for (int u = 0; u < ROW_U; ++u) {
-            f32 v[ROW_E];
-            row_unpack(cur[u], v);
-            const int j = span.first(t + u * ROW_THREADS + tid);
-#pragma unroll
-            for (int e = 0; e < ROW_E; ++e) {
-              const u64 key = st_key(v[e], j + e);
-              best = key > best ? key : best;
-            }
-          }
-          mine = best;
+          for (int u = ROW_U - 1; u >= 0; --u)
+            if (st_order(st_block_max(mb[u])) == st_order(mc)) last = span.first(t + u * ROW_THREADS + tid) + ROW_E - 1;
+          least = st_key(mc, last);
         }
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1) {
-          const u64 o = __shfl_xor_sync(ACC_FULL_MASK, mine, d);
-          mine = o < mine ? o : mine;
+          const u64 o = __shfl_xor_sync(ACC_FULL_MASK, least, d);
+          least = o < least ? o : least;
         }
-        if (lane == 0) sh.key[warp] = mine;
+        if (lane == 0) sh.key[warp] = least;
         __syncthreads();
-        for (int w = 0; w < ST_WARPS; ++w) mine = sh.key[w] < mine ? sh.key[w] : mine;
-        if (mine - 1 > thr_key) thr_key = mine - 1;
+        for (int w = 0; w < ST_WARPS; ++w) least = sh.key[w] < least ? sh.key[w] : least;
+        if (least - 1 > thr_key) thr_key = least - 1;
       }
     }
-    const bool hot = t == b0 ? mc != -ROW_INF : !(mc <= thr);
-    if (__syncthreads_or(hot)) {
-      if (hot) {
+    // Blocks that may hold candidates go to a list; the threads then share its elements.  (The counter alternates:
+    // a fast thread may be listing blocks of the next tile while a slow one reads this tile's count.)
+    if (t == b0 ? mc != -ROW_INF : !(mc <= thr)) {
 #pragma unroll
-        for (int u = 0; u < ROW_U; ++u) {
-#if ROW_F16
-          f32 lo, hi;
-          row_h2x2(mb[u], lo, hi);
-          const f32 bm = row_max_nan(lo, hi);
-#else
-          const f32 bm = mb[u];
-#endif
-          const int j = span.first(t + u * ROW_THREADS + tid);
-          if (t == b0 ? st_order(bm) >= (u32)(thr_key >> 32) : !(bm <= thr)) {
-            f32 v[ROW_E];
-            row_unpack(cur[u], v);
-#pragma unroll
-            for (int e = 0; e < ROW_E; ++e) {
-              const u64 key = st_key(v[e], j + e);
-              if (key > thr_key) {
-                const int slot = atomicAdd(&sh.count, 1);
-                if (slot < ST_CAP) sh.cand[slot] = key;
-              }
-            }
-          }
+      for (int u = 0; u < ROW_U; ++u) {
+        const f32 bm = st_block_max(mb[u]);
+        if (t == b0 ? st_order(bm) >= (u32)(thr_key >> 32) : !(bm <= thr)) {
+          const int slot = atomicAdd(&sh.hot_count[parity], 1);
+          sh.hot[slot] = cur[u];
+          sh.hot_block[slot] = t + u * ROW_THREADS + tid;
         }
+      }
+    }
+    __syncthreads();
+    const int hot = sh.hot_count[parity] * ROW_E;
+    for (int base = 0; base < hot; base += ST_BATCH) {
+      const int end = min(base + ST_BATCH, hot);
+      for (int i = base + tid; i < end; i += ROW_THREADS) {
+        const int slot = i / ROW_E, e = i % ROW_E;
+        const f32 v = row_wide(reinterpret_cast<const row_t*>(&sh.hot[slot])[e]);
+        const u64 key = st_key(v, span.first(sh.hot_block[slot]) + e);
+        if (key > thr_key) sh.cand[atomicAdd(&sh.count, 1)] = key;
       }
       __syncthreads();
-      int total = sh.count;
-      if (total > ST_CAP) {
-        // More candidates than the list holds (a row in rising order): take the tile in pieces of four elements per
-        // thread, and keep the best k of the list after each.
-        __syncthreads();
-        for (int q = 0; q < ROW_U * (ROW_E / 4); ++q) {
-          held = st_compact(sh, held, k);
-          if (held == k) thr_key = sh.cand[k - 1];
-          if (tid == 0) sh.count = held;
-          __syncthreads();
-#pragma unroll
-          for (int u = 0; u < ROW_U; ++u) {
-            f32 v[ROW_E];
-            row_unpack(cur[u], v);
-            const int j = span.first(t + u * ROW_THREADS + tid);
-#pragma unroll
-            for (int e = 0; e < ROW_E; ++e) {
-              if (u * (ROW_E / 4) + e / 4 == q) {
-                const u64 key = st_key(v[e], j + e);
-                if (key > thr_key) sh.cand[atomicAdd(&sh.count, 1)] = key;
-              }
-            }
-          }
-          __syncthreads();
-          held = sh.count;
-          __syncthreads();
-        }
-        total = held;
-      }
-      held = total;
-      if (t == b0 || held > k + 64) {
+      held = sh.count;
+      if (held > (base + ST_BATCH < hot ? ST_CAP - ST_BATCH : (t == b0 ? 0 : k + 64))) {
         held = st_compact(sh, held, k);
         if (held == k) {
           thr_key = sh.cand[k - 1];
           const f32 v = st_value((u32)(thr_key >> 32));
           thr = v != v ? ROW_INF : v;
-        } else {
-          thr_key = ST_NONE;
         }
-        if (tid == 0) sh.count = held;     // (read again only behind the next tile's barriers)
+        if (tid == 0) sh.count = held;
       }
+      __syncthreads();
     }
+    if (hot && tid == 0) sh.hot_count[parity] = 0;
+    parity ^= 1;
 #endif
   }
 #if ROW_TOPK

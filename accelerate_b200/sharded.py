@@ -81,6 +81,16 @@ class ProgramCache:
         return ent[:3]
 
 
+class _View:
+    """One leaf of a device array, described the way torch takes other libraries' device memory."""
+
+    def __init__(self, a, leaf):
+        self.__cuda_array_interface__ = {"shape": a.shape or (1,), "typestr": _TYPESTR[a.leaf_types[leaf]], "data": (a.devptr(leaf), False), "version": 3}
+
+
+_TYPESTR = {t: np.dtype(d).str for t, d in L.NP_OF.items()}
+
+
 class GpuExecutor:
     """Runs terms on this rank's GPU; arrays are ``backend.DeviceArray``."""
 
@@ -130,22 +140,18 @@ class GpuExecutor:
 
     def tensor(self, a, leaf=0):
         """Zero-copy torch view of one leaf of a device array."""
-        dt = np.dtype(L.NP_OF[a.leaf_types[leaf]])
-        n = int(np.prod(a.shape)) if len(a.shape) else 1
-        if n == 0:
+        if 0 in a.shape:
+            dt = np.dtype(L.NP_OF[a.leaf_types[leaf]])
             return torch.empty(a.shape, dtype=torch.from_numpy(np.empty(0, dt)).dtype, device=self.stream.device)
-
-        class View:
-            pass
-        v = View()
-        v.__cuda_array_interface__ = {"shape": tuple(a.shape) if len(a.shape) else (1,), "typestr": dt.str, "data": (a.devptr(leaf), False),
-                                      "version": 3}
-        t = torch.as_tensor(v, device=self.stream.device)
+        t = torch.as_tensor(_View(a, leaf), device=self.stream.device)
         t._keepalive = a
         return t
 
     def wrap(self, t, elt):
-        """Device array over a torch tensor's memory (the tensor must stay alive)."""
+        """Device array over a torch tensor's memory (the tensor must stay alive).  Arrays are dense, so the tensor
+        must be contiguous."""
+        if not t.is_contiguous():
+            raise ValueError("only a contiguous tensor can be an array's memory")
         a = self.ctx.wrap(elt, tuple(t.shape), [t.data_ptr()])
         a._keepalive = t
         return a

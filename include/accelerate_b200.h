@@ -98,6 +98,9 @@ int b200_array_shape(b200_ctx* ctx, uint64_t id, int64_t* shape);
 int b200_array_num_leaves(b200_ctx* ctx, uint64_t id, int* n);
 /* Scalar type name of a leaf ("f32", ...); pointer valid for the process lifetime. */
 int b200_array_leaf_type(b200_ctx* ctx, uint64_t id, int leaf, const char** name);
+/* The same in one call: rank and extents, number of leaves and their scalar types (0.. in the order i8 i16 i32 i64 u8 u16
+ * u32 u64 f32 f64 f16).  B200_ERR_ARG if `shape` has room for fewer than `rank` extents or `types` for fewer leaves. */
+int b200_array_info(b200_ctx* ctx, uint64_t id, int max_rank, int* rank, int64_t* shape, int max_leaves, int* leaves, int32_t* types);
 int b200_array_devptr(b200_ctx* ctx, uint64_t id, int leaf, void** ptr);
 
 /* Load a program: the text serialisation of a DelayedAfun (Trafo/Delayed.hs:41-60),
