@@ -131,9 +131,9 @@ Glue foreign_glue(const Node& n) {
 // ---- launch shapes ------------------------------------------------------------------------------------
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256, kStatsThreads = 128;
 
-Variant stats_variant(int ctas) { return {{"ROW_THREADS", str(kThreads)}, {"ROW_U", "4"}, {"ROW_MIN_BLOCKS", "3"}, {"ROW_C", str(ctas)}}; }
+Variant stats_variant(int ctas) { return {{"ROW_THREADS", str(kStatsThreads)}, {"ROW_U", "8"}, {"ROW_MIN_BLOCKS", "6"}, {"ROW_C", str(ctas)}}; }
 Variant distill_grad_variant(int ctas) { return {{"ROW_THREADS", str(kThreads)}, {"ROW_U", "4"}, {"ROW_MIN_BLOCKS", "4"}, {"ROW_C", str(ctas)}}; }
 
 // CTAs that share a row: enough to give every SM several, as long as each has a tile of its own
@@ -270,8 +270,8 @@ void Program::exec_foreign(const Node& n, Env& env) {
       env[n.outs[1]] = top;
       if (rows == 0) break;
       const int ctas = ctas_per_row(rows, cols, elt_bytes, c.sm_count, 8);
-      CompiledKernel& ker = shape_kernel(c, st, (uint64_t)ctas, "rows_stats", [&] { return stats_variant(ctas); }, "acc_rows_stats", kThreads, 0);
-      launch(c, ker, rows * ctas, kThreads, 0,
+      CompiledKernel& ker = shape_kernel(c, st, (uint64_t)ctas, "rows_stats", [&] { return stats_variant(ctas); }, "acc_rows_stats", kStatsThreads, 0);
+      launch(c, ker, rows * ctas, kStatsThreads, 0,
              {ptr_of(x), ptr_of(*a[0]), 0, ptr_of(*stats, 0), ptr_of(*stats, 1), ptr_of(*stats, 2), ptr_of(*top, 0), ptr_of(*top, 1),
               (uint64_t)rows, (uint64_t)cols, (uint64_t)k, float_bits(1.0), err});
       break;
@@ -288,8 +288,8 @@ void Program::exec_foreign(const Node& n, Env& env) {
         env[n.outs[1]] = lse;
         if (rows == 0) break;
         const int ctas = ctas_per_row(rows, cols, elt_bytes, c.sm_count, 8);
-        CompiledKernel& ker = shape_kernel(c, st, (uint64_t)ctas, "rows_stats", [&] { return stats_variant(ctas); }, "acc_rows_stats", kThreads, 0);
-        launch(c, ker, rows * ctas, kThreads, 0,
+        CompiledKernel& ker = shape_kernel(c, st, (uint64_t)ctas, "rows_stats", [&] { return stats_variant(ctas); }, "acc_rows_stats", kStatsThreads, 0);
+        launch(c, ker, rows * ctas, kStatsThreads, 0,
                {ptr_of(x), ptr_of(*a[0]), ptr_of(*a[1]), ptr_of(*loss), ptr_of(*lse), 0, 0, 0, (uint64_t)rows, (uint64_t)cols, (uint64_t)k,
                 float_bits(n.consts[0]), err});
       } else {

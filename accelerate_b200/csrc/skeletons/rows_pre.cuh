@@ -76,18 +76,38 @@ struct row_span {
   __device__ __forceinline__ uint4 load(int i) const {
     const int j = first(i);
     if (j >= 0 && j + ROW_E <= n) return __ldcs(reinterpret_cast<const uint4*>(x + j));
-    u32 w[4] = {ROW_PAD, ROW_PAD, ROW_PAD, ROW_PAD};
-#pragma unroll
-    for (int e = 0; e < ROW_E; ++e)
-      if (j + e >= 0 && j + e < n) {
+    u64 w[2] = {(u64)ROW_PAD << 32 | ROW_PAD, (u64)ROW_PAD << 32 | ROW_PAD};
+    constexpr int BITS = 8 * (int)sizeof(row_t);
+    const int e0 = j < 0 ? -j : 0, e1 = min(ROW_E, n - j);
+#pragma unroll 1
+    for (int e = e0; e < e1; ++e) {
 #if ROW_F16
-        const u32 h = x[j + e];
-        w[e / 2] = (e & 1) ? ((w[e / 2] & 0x0000ffffu) | (h << 16)) : ((w[e / 2] & 0xffff0000u) | h);
+      const u64 h = x[j + e];
 #else
-        w[e] = __float_as_uint(x[j + e]);
+      const u64 h = __float_as_uint(x[j + e]);
 #endif
-      }
-    return make_uint4(w[0], w[1], w[2], w[3]);
+      const int at = e * BITS & 63;
+      const u64 mask = (((u64)1 << BITS) - 1) << at;
+      if (e * BITS < 64) w[0] = (w[0] & ~mask) | (h << at);
+      else w[1] = (w[1] & ~mask) | (h << at);
+    }
+    return make_uint4((u32)w[0], (u32)(w[0] >> 32), (u32)w[1], (u32)(w[1] >> 32));
+  }
+  // The blocks that lie wholly inside the row: [inner0, inner1)
+  __device__ __forceinline__ int inner0() const { return shift ? 1 : 0; }
+  __device__ __forceinline__ int inner1() const { return (shift + n) / ROW_E; }
+  // Block i of those
+  __device__ __forceinline__ uint4 load_inner(int i) const { return __ldcs(reinterpret_cast<const uint4*>(x - shift) + i); }
+  // U blocks per thread, THREADS apart, from block t on; blocks from `end` on read as -inf
+  template <int U> __device__ __forceinline__ void load_tile(uint4 (&b)[U], int t, int end) const {
+    const int i = t + (int)threadIdx.x;
+    if (t >= inner0() && t + U * ROW_THREADS <= min(end, inner1())) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) b[u] = load_inner(i + u * ROW_THREADS);
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u) b[u] = i + u * ROW_THREADS < end ? load(i + u * ROW_THREADS) : make_uint4(ROW_PAD, ROW_PAD, ROW_PAD, ROW_PAD);
+    }
   }
 };
 

@@ -20,18 +20,19 @@ struct Params { i64 x, tok, teacher, out0, out1, out2, out3, out4, rows, n, k, t
 
 constexpr int ST_TILE = ROW_THREADS * ROW_U;     // blocks per tile
 constexpr int ST_WARPS = ROW_THREADS / 32;
-constexpr int ST_CAP = 2048;                     // candidate keys held in shared memory
+constexpr int ST_CAP = 1024;                     // candidate keys held in shared memory
 constexpr int ST_BATCH = ST_CAP / 2;             // elements looked at between two looks at the list
+constexpr int ST_HOT = 512;                      // listed blocks
 
 struct row_stat { f32 m, z, w; };
 struct st_shared {
 #if ROW_TOPK
-  u64 cand[ST_CAP];
-  uint4 hot[ST_TILE];  // blocks of the tile that may hold candidates,
-  int hot_block[ST_TILE];  // and their numbers
-  int hot_count[2];    // of this tile and the next
-  int count;           // candidates, while they are being appended
-  int kept;            // candidates of this CTA at the end (read by the cluster's first CTA)
+  __align__(16) u64 cand[ST_CAP];
+  uint4 hot[ST_HOT];        // blocks that may hold candidates,
+  int hot_block[ST_HOT];    // and their numbers
+  int hot_count;
+  int count;                // candidates, while they are being appended
+  int kept;                 // candidates of this CTA at the end (read by the cluster's first CTA)
   u64 key[ST_WARPS];
 #endif
   row_stat part[ST_WARPS];
@@ -82,8 +83,8 @@ __device__ __forceinline__ f32 st_block_max(f32 m) { return m; }
 
 #if ROW_TOPK
 // The best k of the n candidates, in falling order, to the front of the list; returns how many there are.
-// Up to one candidate per thread: each counts the candidates above its own.  More (only rows in an unusual
-// order, or lists of many CTAs): a bitonic sort.
+// Up to four candidates per thread: each thread counts the candidates above its own.  More (rows in an unusual
+// order, lists of many CTAs): a bitonic sort.
 __device__ __forceinline__ int st_compact(st_shared& sh, int n, int k) {
   const int tid = threadIdx.x;
   if (n <= ROW_THREADS) {
@@ -91,19 +92,37 @@ __device__ __forceinline__ int st_compact(st_shared& sh, int n, int k) {
     int rank = 0;
     if ((tid & ~31) < n) {
       key = tid < n ? sh.cand[tid] : 0;
-      for (int i = 0; i < n; ++i) rank += sh.cand[i] > key ? 1 : 0;
+      int i = 0;
+      for (; i + 4 <= n; i += 4) {
+        const ulonglong2 a = *reinterpret_cast<const ulonglong2*>(&sh.cand[i]), b = *reinterpret_cast<const ulonglong2*>(&sh.cand[i + 2]);
+        rank += (a.x > key) + (a.y > key) + (b.x > key) + (b.y > key);
+      }
+      for (; i < n; ++i) rank += sh.cand[i] > key;
     }
     __syncthreads();
     if (tid < n && rank < k) sh.cand[rank] = key;
     __syncthreads();
-  } else {
-    int size = ROW_THREADS;
-    while (size < n) size <<= 1;
-    for (int i = n + tid; i < size; i += ROW_THREADS) sh.cand[i] = 0;
+  } else if (n <= 4 * ROW_THREADS) {
+    u64 key[4];
+    int rank[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int q = 0; q < 4; ++q) key[q] = q * ROW_THREADS + tid < n ? sh.cand[q * ROW_THREADS + tid] : 0;
+    for (int i = 0; i < n; ++i) {
+      const u64 c = sh.cand[i];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) rank[q] += c > key[q];
+    }
     __syncthreads();
-    for (int len = 2; len <= size; len <<= 1)
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (q * ROW_THREADS + tid < n && rank[q] < k) sh.cand[rank[q]] = key[q];
+    __syncthreads();
+  } else {
+    for (int i = n + tid; i < ST_CAP; i += ROW_THREADS) sh.cand[i] = 0;
+    __syncthreads();
+    for (int len = 2; len <= ST_CAP; len <<= 1)
       for (int d = len >> 1; d > 0; d >>= 1) {
-        for (int i = tid; i < size / 2; i += ROW_THREADS) {
+        for (int i = tid; i < ST_CAP / 2; i += ROW_THREADS) {
           const int lo = 2 * i - (i & (d - 1)), hi = lo + d;
           const u64 a = sh.cand[lo], b = sh.cand[hi];
           const bool falling = (lo & len) == 0;
@@ -113,6 +132,62 @@ __device__ __forceinline__ int st_compact(st_shared& sh, int n, int k) {
       }
   }
   return n < k ? n : k;
+}
+
+// The candidate list of a CTA, the same in every thread
+struct st_list {
+  int held = 0;                  // candidates
+  u64 thr_key = ST_NONE;         // only elements above this key are candidates
+  f32 thr = -ROW_INF;            // its value: a quick test for all elements of a thread
+};
+// A block that may hold a candidate goes to the list of blocks.  Its best possible key: the block's maximum at the
+// block's first element.
+__device__ __forceinline__ void st_push(st_shared& sh, const st_list& l, const uint4& block, f32 most, int i, int first) {
+  if (st_key(most, max(first, 0)) > l.thr_key) {
+    const int slot = atomicAdd(&sh.hot_count, 1);
+    if (slot < ST_HOT) {
+      sh.hot[slot] = block;
+      sh.hot_block[slot] = i;
+    }
+  }
+}
+// The threads share the listed blocks' elements; those above the threshold become candidates, and the best k of them
+// the new list.  False, and nothing done, if more blocks came than the list holds.
+__device__ __forceinline__ bool st_drain(st_shared& sh, st_list& l, const row_span& span, int k) {
+  const int tid = threadIdx.x;
+  __syncthreads();
+  const int blocks = sh.hot_count;
+  __syncthreads();
+  if (tid == 0) sh.hot_count = 0;        // (seen by whoever lists the next block: a barrier follows on every way)
+  if (blocks > ST_HOT) {
+    __syncthreads();
+    return false;
+  }
+  const int n = blocks * ROW_E;
+  for (int base = 0; base < n; base += ST_BATCH) {
+    const int end = min(base + ST_BATCH, n);
+    for (int i = base + tid; i < end; i += ROW_THREADS) {
+      const int slot = i / ROW_E, e = i % ROW_E;
+      const f32 v = row_wide(reinterpret_cast<const row_t*>(&sh.hot[slot])[e]);
+      const u64 key = st_key(v, span.first(sh.hot_block[slot]) + e);
+      if (key > l.thr_key) sh.cand[atomicAdd(&sh.count, 1)] = key;
+    }
+    __syncthreads();
+    l.held = sh.count;
+    if (base + ST_BATCH < n ? l.held > ST_CAP - ST_BATCH : l.held > 0) {
+      l.held = st_compact(sh, l.held, k);
+      if (l.held == k) {
+        l.thr_key = sh.cand[k - 1];
+        const f32 v = st_value((u32)(l.thr_key >> 32));
+        l.thr = v != v ? ROW_INF : v;
+      }
+    }
+    __syncthreads();
+    if (tid == 0) sh.count = l.held;
+    __syncthreads();
+  }
+  if (n == 0) __syncthreads();
+  return true;
 }
 #endif
 
@@ -144,31 +219,15 @@ acc_rows_stats(const __grid_constant__ Params p) {
 
   row_stat st = {-ROW_INF, 0.0f, 0.0f};
 #if ROW_TOPK
-  int held = 0;                         // candidates in the list (the same in every thread)
-  u64 thr_key = ST_NONE;                // only elements above this key are candidates
-  f32 thr = -ROW_INF;                   // its value: a quick test for a whole chunk
-  int parity = 0;
-  if (tid == 0) sh.count = sh.hot_count[0] = sh.hot_count[1] = 0;
+  st_list list;
+  int drained = b0, due = b0;            // tiles from `drained` on have blocks in the list; it is drained behind tile `due`
+  if (tid == 0) sh.count = sh.hot_count = 0;
   __syncthreads();
 #endif
 
-  uint4 cur[ROW_U], nxt[ROW_U];
-  const uint4 pad = make_uint4(ROW_PAD, ROW_PAD, ROW_PAD, ROW_PAD);
-#pragma unroll
-  for (int u = 0; u < ROW_U; ++u) {
-    const int i = b0 + u * ROW_THREADS + tid;
-    nxt[u] = i < b1 ? span.load(i) : pad;
-  }
   for (int t = b0; t < b1; t += ST_TILE) {
-#pragma unroll
-    for (int u = 0; u < ROW_U; ++u) cur[u] = nxt[u];
-    if (t + ST_TILE < b1) {
-#pragma unroll
-      for (int u = 0; u < ROW_U; ++u) {
-        const int i = t + ST_TILE + u * ROW_THREADS + tid;
-        nxt[u] = i < b1 ? span.load(i) : pad;
-      }
-    }
+    uint4 cur[ROW_U];
+    span.load_tile(cur, t, b1);
     // maxima: of each block and of the chunk (a NaN stays visible)
     f32 mc;
 #if ROW_F16
@@ -261,51 +320,48 @@ acc_rows_stats(const __grid_constant__ Params p) {
         if (lane == 0) sh.key[warp] = least;
         __syncthreads();
         for (int w = 0; w < ST_WARPS; ++w) least = sh.key[w] < least ? sh.key[w] : least;
-        if (least - 1 > thr_key) thr_key = least - 1;
+        if (least - 1 > list.thr_key) list.thr_key = least - 1;
       }
     }
-    // Blocks that may hold candidates go to a list; the threads then share its elements.  (The counter alternates:
-    // a fast thread may be listing blocks of the next tile while a slow one reads this tile's count.)
-    if (t == b0 ? mc != -ROW_INF : !(mc <= thr)) {
+    // (later elements of the threshold's own value stand behind it: their indices are higher)
+    if (t == b0 ? mc != -ROW_INF : !(mc <= list.thr)) {
 #pragma unroll
       for (int u = 0; u < ROW_U; ++u) {
-        const f32 bm = st_block_max(mb[u]);
-        if (t == b0 ? st_order(bm) >= (u32)(thr_key >> 32) : !(bm <= thr)) {
-          const int slot = atomicAdd(&sh.hot_count[parity], 1);
-          sh.hot[slot] = cur[u];
-          sh.hot_block[slot] = t + u * ROW_THREADS + tid;
-        }
+        const int i = t + u * ROW_THREADS + tid;
+        st_push(sh, list, cur[u], st_block_max(mb[u]), i, span.first(i));
       }
     }
-    __syncthreads();
-    const int hot = sh.hot_count[parity] * ROW_E;
-    for (int base = 0; base < hot; base += ST_BATCH) {
-      const int end = min(base + ST_BATCH, hot);
-      for (int i = base + tid; i < end; i += ROW_THREADS) {
-        const int slot = i / ROW_E, e = i % ROW_E;
-        const f32 v = row_wide(reinterpret_cast<const row_t*>(&sh.hot[slot])[e]);
-        const u64 key = st_key(v, span.first(sh.hot_block[slot]) + e);
-        if (key > thr_key) sh.cand[atomicAdd(&sh.count, 1)] = key;
-      }
-      __syncthreads();
-      held = sh.count;
-      if (held > (base + ST_BATCH < hot ? ST_CAP - ST_BATCH : (t == b0 ? 0 : k + 64))) {
-        held = st_compact(sh, held, k);
-        if (held == k) {
-          thr_key = sh.cand[k - 1];
-          const f32 v = st_value((u32)(thr_key >> 32));
-          thr = v != v ? ROW_INF : v;
+    // The list is drained behind the first tile and whenever the part of the row seen since has doubled: each time
+    // about k elements are expected above the old threshold.  Warps run on their own in between.
+    if (t >= due || t + ST_TILE >= b1) {
+      if (!st_drain(sh, list, span, k)) {
+        // More blocks than the list holds (a row in rising order): once more over the same tiles, with the list
+        // drained as often as it may fill up.
+        const int end = min(t + ST_TILE, b1);
+        for (int s = drained; s < end; s += ST_HOT) {
+#pragma unroll 1
+          for (int u = 0; u < ST_HOT / ROW_THREADS; ++u) {
+            const int i = s + u * ROW_THREADS + tid;
+            if (i < end) {
+              const uint4 block = span.load(i);
+              f32 v[ROW_E], most;
+              row_unpack(block, v);
+              most = v[0];
+#pragma unroll
+              for (int e = 1; e < ROW_E; ++e) most = row_max_nan(most, v[e]);
+              st_push(sh, list, block, most, i, span.first(i));
+            }
+          }
+          st_drain(sh, list, span, k);
         }
-        if (tid == 0) sh.count = held;
       }
-      __syncthreads();
+      drained = t + ST_TILE;
+      due = drained + (drained - b0) - ST_TILE;
     }
-    if (hot && tid == 0) sh.hot_count[parity] = 0;
-    parity ^= 1;
 #endif
   }
 #if ROW_TOPK
-  held = st_compact(sh, held, k);
+  int held = list.held;                  // (sorted by the last drain)
   if (tid == 0) sh.kept = held;
 #endif
   // join the statistics: lanes, warps, CTAs of the cluster
@@ -420,19 +476,24 @@ acc_rows_stats(const __grid_constant__ Params p) {
   __syncthreads();
   if (held < k) {
     // All elements above -inf are in the list.  The places behind them go to -inf elements, lowest index first: they
-    // are among the row's first 2k - 1 (at most 255) elements.
-    bool free_one = tid < n && tid < 2 * k;
-    for (int i = 0; i < held; ++i) free_one = free_one && st_index(sh.cand[i]) != tid;
-    const u32 ones = __ballot_sync(ACC_FULL_MASK, free_one);
-    if (lane == 0) sh.warp_count[warp] = __popc(ones);
-    __syncthreads();
-    int at = held + __popc(ones & ((1u << lane) - 1)), all = held;
-    for (int w = 0; w < ST_WARPS; ++w) {
-      if (w < warp) at += sh.warp_count[w];
-      all += sh.warp_count[w];
+    // are among the row's first 2k - 1 elements.
+    const int finite = held;
+    for (int base = 0; base < 2 * k; base += ROW_THREADS) {
+      const int j = base + tid;
+      bool free_one = j < n && j < 2 * k;
+      for (int i = 0; i < finite; ++i) free_one = free_one && st_index(sh.cand[i]) != j;
+      const u32 ones = __ballot_sync(ACC_FULL_MASK, free_one);
+      __syncthreads();
+      if (lane == 0) sh.warp_count[warp] = __popc(ones);
+      __syncthreads();
+      int at = held + __popc(ones & ((1u << lane) - 1)), all = held;
+      for (int w = 0; w < ST_WARPS; ++w) {
+        if (w < warp) at += sh.warp_count[w];
+        all += sh.warp_count[w];
+      }
+      if (free_one && at < k) sh.cand[at] = st_key(-ROW_INF, j);
+      held = all < k ? all : k;
     }
-    if (free_one && at < k) sh.cand[at] = st_key(-ROW_INF, tid);
-    held = all < k ? all : k;
     __syncthreads();
   }
   if (tid < k) {
