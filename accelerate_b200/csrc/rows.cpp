@@ -47,6 +47,9 @@ const ArrayInfo& rows_arg(const Node& n) {
 std::string ctype(Ty t) { return t == F16 ? "u16" : t == F32 ? "f32" : t == I64 ? "i64" : "i32"; }
 std::string str(int64_t v) { return std::to_string(v); }
 
+// what the kernel's st_shared takes (rows_stats.cuh): candidates and listed blocks, and the warps' statistics
+size_t stats_smem(bool topk) { return (topk ? 1024 * 8 + 512 * 20 : 0) + 512; }
+
 }  // namespace
 
 Foreign foreign_named(const std::string& name) {
@@ -114,11 +117,13 @@ Glue foreign_glue(const Node& n) {
     case F_LOG_PROBS:
       g.defines["ROW_DISTILL"] = "0";
       g.defines["ROW_TOPK"] = n.consts[0] > 0 ? "1" : "0";
+      g.defines["ROW_SMEM"] = str((int64_t)stats_smem(n.consts[0] > 0));
       g.code = "typedef " + ctype(n.arg_info[0].elt.s) + " token_t;\n";
       break;
     case F_DISTILL:
       g.defines["ROW_DISTILL"] = "1";
       g.defines["ROW_TOPK"] = "0";
+      g.defines["ROW_SMEM"] = str((int64_t)stats_smem(false));
       g.code = "typedef " + ctype(n.arg_info[1].elt.s) + " teacher_t;\n";
       break;
     case F_DISTILL_GRAD: g.code = "typedef " + ctype(n.arg_info[1].elt.s) + " teacher_t;\n"; break;
@@ -133,7 +138,7 @@ namespace {
 
 constexpr int kThreads = 256, kStatsThreads = 128;
 
-Variant stats_variant(int ctas) { return {{"ROW_THREADS", str(kStatsThreads)}, {"ROW_U", "8"}, {"ROW_MIN_BLOCKS", "6"}, {"ROW_C", str(ctas)}}; }
+Variant stats_variant(int ctas) { return {{"ROW_THREADS", str(kStatsThreads)}, {"ROW_U", "8"}, {"ROW_MIN_BLOCKS", "7"}, {"ROW_C", str(ctas)}}; }
 Variant distill_grad_variant(int ctas) { return {{"ROW_THREADS", str(kThreads)}, {"ROW_U", "4"}, {"ROW_MIN_BLOCKS", "4"}, {"ROW_C", str(ctas)}}; }
 
 // CTAs that share a row: enough to give every SM several, as long as each has a tile of its own
@@ -270,8 +275,9 @@ void Program::exec_foreign(const Node& n, Env& env) {
       env[n.outs[1]] = top;
       if (rows == 0) break;
       const int ctas = ctas_per_row(rows, cols, elt_bytes, c.sm_count, 8);
-      CompiledKernel& ker = shape_kernel(c, st, (uint64_t)ctas, "rows_stats", [&] { return stats_variant(ctas); }, "acc_rows_stats", kStatsThreads, 0);
-      launch(c, ker, rows * ctas, kStatsThreads, 0,
+      const size_t smem = stats_smem(k > 0);
+      CompiledKernel& ker = shape_kernel(c, st, (uint64_t)ctas, "rows_stats", [&] { return stats_variant(ctas); }, "acc_rows_stats", kStatsThreads, smem);
+      launch(c, ker, rows * ctas, kStatsThreads, smem,
              {ptr_of(x), ptr_of(*a[0]), 0, ptr_of(*stats, 0), ptr_of(*stats, 1), ptr_of(*stats, 2), ptr_of(*top, 0), ptr_of(*top, 1),
               (uint64_t)rows, (uint64_t)cols, (uint64_t)k, float_bits(1.0), err});
       break;
@@ -288,8 +294,9 @@ void Program::exec_foreign(const Node& n, Env& env) {
         env[n.outs[1]] = lse;
         if (rows == 0) break;
         const int ctas = ctas_per_row(rows, cols, elt_bytes, c.sm_count, 8);
-        CompiledKernel& ker = shape_kernel(c, st, (uint64_t)ctas, "rows_stats", [&] { return stats_variant(ctas); }, "acc_rows_stats", kStatsThreads, 0);
-        launch(c, ker, rows * ctas, kStatsThreads, 0,
+        const size_t smem = stats_smem(false);
+        CompiledKernel& ker = shape_kernel(c, st, (uint64_t)ctas, "rows_stats", [&] { return stats_variant(ctas); }, "acc_rows_stats", kStatsThreads, smem);
+        launch(c, ker, rows * ctas, kStatsThreads, smem,
                {ptr_of(x), ptr_of(*a[0]), ptr_of(*a[1]), ptr_of(*loss), ptr_of(*lse), 0, 0, 0, (uint64_t)rows, (uint64_t)cols, (uint64_t)k,
                 float_bits(n.consts[0]), err});
       } else {

@@ -30,7 +30,7 @@ struct st_shared {
   __align__(16) u64 cand[ST_CAP];
   uint4 hot[ST_HOT];        // blocks that may hold candidates,
   int hot_block[ST_HOT];    // and their numbers
-  int hot_count;
+  int hot_count[2];         // of this list and the next
   int count;                // candidates, while they are being appended
   int kept;                 // candidates of this CTA at the end (read by the cluster's first CTA)
   u64 key[ST_WARPS];
@@ -39,6 +39,11 @@ struct st_shared {
   row_stat cta;
   int warp_count[ST_WARPS];
 };
+
+
+extern __shared__ uint4 st_memory[];
+static_assert(sizeof(st_shared) <= ROW_SMEM, "the host asks for less shared memory than the kernel uses");
+#define sh (*reinterpret_cast<st_shared*>(st_memory))
 
 // (a maximum of -inf, "nothing yet", stands at 0: its sums are 0)
 __device__ __forceinline__ f32 st_base(f32 m) { return m == -ROW_INF ? 0.0f : m; }
@@ -82,41 +87,51 @@ __device__ __forceinline__ f32 st_block_max(f32 m) { return m; }
 #define ST_NONE ((u64)0x007fffffffffffffull)     /* the best key of a -inf element: candidates lie above it */
 
 #if ROW_TOPK
-// The best k of the n candidates, in falling order, to the front of the list; returns how many there are.
-// Up to four candidates per thread: each thread counts the candidates above its own.  More (rows in an unusual
-// order, lists of many CTAs): a bitonic sort.
-__device__ __forceinline__ int st_compact(st_shared& sh, int n, int k) {
+// Every candidate to its place in falling order, as long as that is one of the first k; `sorted` of the n candidates are
+// in order already, at the front.  A thread counts, for Q candidates, those among the unsorted ones that are better;
+// among the sorted ones a search finds the place.
+template <int Q> __device__ __forceinline__ void st_rank(int sorted, int n, int k) {
   const int tid = threadIdx.x;
-  if (n <= ROW_THREADS) {
-    u64 key = 0;
-    int rank = 0;
-    if ((tid & ~31) < n) {
-      key = tid < n ? sh.cand[tid] : 0;
-      int i = 0;
-      for (; i + 4 <= n; i += 4) {
-        const ulonglong2 a = *reinterpret_cast<const ulonglong2*>(&sh.cand[i]), b = *reinterpret_cast<const ulonglong2*>(&sh.cand[i + 2]);
-        rank += (a.x > key) + (a.y > key) + (b.x > key) + (b.y > key);
-      }
-      for (; i < n; ++i) rank += sh.cand[i] > key;
-    }
-    __syncthreads();
-    if (tid < n && rank < k) sh.cand[rank] = key;
-    __syncthreads();
-  } else if (n <= 4 * ROW_THREADS) {
-    u64 key[4];
-    int rank[4] = {0, 0, 0, 0};
+  u64 key[Q];
+  int rank[Q];
+  if (sorted <= 32) sorted = 0;          // (counting through them is no slower than the search)
+  if ((tid & ~31) < n) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) key[q] = q * ROW_THREADS + tid < n ? sh.cand[q * ROW_THREADS + tid] : 0;
-    for (int i = 0; i < n; ++i) {
+    for (int q = 0; q < Q; ++q) {
+      const int i = q * ROW_THREADS + tid;
+      key[q] = i < n ? sh.cand[i] : 0;
+      rank[q] = i < sorted ? i : 0;
+      if (i >= sorted) {
+        int lo = 0, hi = sorted;         // better ones: [0, lo), worse ones: [hi, sorted)
+        while (lo < hi) {
+          const int mid = (lo + hi) >> 1;
+          if (sh.cand[mid] > key[q]) lo = mid + 1; else hi = mid;
+        }
+        rank[q] = lo;
+      }
+    }
+#pragma unroll 4
+    for (int i = sorted; i < n; ++i) {
       const u64 c = sh.cand[i];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) rank[q] += c > key[q];
+      for (int q = 0; q < Q; ++q) rank[q] += c > key[q];
     }
-    __syncthreads();
+  }
+  __syncthreads();
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
-      if (q * ROW_THREADS + tid < n && rank[q] < k) sh.cand[rank[q]] = key[q];
-    __syncthreads();
+  for (int q = 0; q < Q; ++q)
+    if (q * ROW_THREADS + tid < n && rank[q] < k) sh.cand[rank[q]] = key[q];
+  if (tid == 0) sh.count = n < k ? n : k;
+  __syncthreads();
+}
+// The best k of the n candidates, in falling order, to the front of the list, and their number.  Long lists
+// (rows in an unusual order): a bitonic sort.
+__device__ __forceinline__ int st_compact(int sorted, int n, int k) {
+  const int tid = threadIdx.x;
+  if (n <= ROW_THREADS) {
+    st_rank<1>(sorted, n, k);
+  } else if (n <= 2 * ROW_THREADS) {
+    st_rank<2>(sorted, n, k);
   } else {
     for (int i = n + tid; i < ST_CAP; i += ROW_THREADS) sh.cand[i] = 0;
     __syncthreads();
@@ -130,6 +145,8 @@ __device__ __forceinline__ int st_compact(st_shared& sh, int n, int k) {
         }
         __syncthreads();
       }
+    if (tid == 0) sh.count = n < k ? n : k;
+    __syncthreads();
   }
   return n < k ? n : k;
 }
@@ -137,14 +154,26 @@ __device__ __forceinline__ int st_compact(st_shared& sh, int n, int k) {
 // The candidate list of a CTA, the same in every thread
 struct st_list {
   int held = 0;                  // candidates
+  int sorted = 0;                // so many of them, at the front, are in order
+  bool overflow = false;
+  int phase = 0;                 // which count the blocks listed now go to
   u64 thr_key = ST_NONE;         // only elements above this key are candidates
   f32 thr = -ROW_INF;            // its value: a quick test for all elements of a thread
+#if ROW_F16
+  u32 thr2 = ROW_PAD;            // the same as two Halves (every threshold is an element, so this is exact)
+#endif
 };
+// Whether a block's maximum is above the threshold's value, or NaN
+#if ROW_F16
+__device__ __forceinline__ bool st_above(u32 most, const st_list& l) { return row_max_nan2(most, l.thr2) != l.thr2; }
+#else
+__device__ __forceinline__ bool st_above(f32 most, const st_list& l) { return !(most <= l.thr); }
+#endif
 // A block that may hold a candidate goes to the list of blocks.  Its best possible key: the block's maximum at the
 // block's first element.
-__device__ __forceinline__ void st_push(st_shared& sh, const st_list& l, const uint4& block, f32 most, int i, int first) {
+__device__ __forceinline__ void st_push(const st_list& l, const uint4& block, f32 most, int i, int first) {
   if (st_key(most, max(first, 0)) > l.thr_key) {
-    const int slot = atomicAdd(&sh.hot_count, 1);
+    const int slot = atomicAdd(&sh.hot_count[l.phase], 1);
     if (slot < ST_HOT) {
       sh.hot[slot] = block;
       sh.hot_block[slot] = i;
@@ -152,16 +181,19 @@ __device__ __forceinline__ void st_push(st_shared& sh, const st_list& l, const u
   }
 }
 // The threads share the listed blocks' elements; those above the threshold become candidates, and the best k of them
-// the new list.  False, and nothing done, if more blocks came than the list holds.
-__device__ __forceinline__ bool st_drain(st_shared& sh, st_list& l, const row_span& span, int k) {
+// the new list.  `overflow`, and nothing done, if more blocks came than the list holds.
+__device__ __forceinline__ st_list st_drain(st_list l, int shift, int k) {
   const int tid = threadIdx.x;
   __syncthreads();
-  const int blocks = sh.hot_count;
-  __syncthreads();
-  if (tid == 0) sh.hot_count = 0;        // (seen by whoever lists the next block: a barrier follows on every way)
-  if (blocks > ST_HOT) {
+  // (the other count is 0: it was cleared a drain ago, with barriers since)
+  const int blocks = sh.hot_count[l.phase];
+  l.phase ^= 1;
+  l.overflow = blocks > ST_HOT;
+  if (blocks == 0) return l;
+  if (l.overflow) {
     __syncthreads();
-    return false;
+    if (tid == 0) sh.hot_count[l.phase ^ 1] = 0;
+    return l;
   }
   const int n = blocks * ROW_E;
   for (int base = 0; base < n; base += ST_BATCH) {
@@ -169,25 +201,28 @@ __device__ __forceinline__ bool st_drain(st_shared& sh, st_list& l, const row_sp
     for (int i = base + tid; i < end; i += ROW_THREADS) {
       const int slot = i / ROW_E, e = i % ROW_E;
       const f32 v = row_wide(reinterpret_cast<const row_t*>(&sh.hot[slot])[e]);
-      const u64 key = st_key(v, span.first(sh.hot_block[slot]) + e);
+      const u64 key = st_key(v, sh.hot_block[slot] * ROW_E - shift + e);
       if (key > l.thr_key) sh.cand[atomicAdd(&sh.count, 1)] = key;
     }
     __syncthreads();
     l.held = sh.count;
-    if (base + ST_BATCH < n ? l.held > ST_CAP - ST_BATCH : l.held > 0) {
-      l.held = st_compact(sh, l.held, k);
-      if (l.held == k) {
-        l.thr_key = sh.cand[k - 1];
-        const f32 v = st_value((u32)(l.thr_key >> 32));
-        l.thr = v != v ? ROW_INF : v;
-      }
+    if (base + ST_BATCH < n) {
+      if (l.held > ST_CAP - ST_BATCH) l.held = l.sorted = st_compact(l.sorted, l.held, k);
+      else __syncthreads();              // (everybody has read the count)
+    } else {
+      if (tid == 0) sh.hot_count[l.phase ^ 1] = 0;
+      l.held = l.sorted = st_compact(l.sorted, l.held, k);
     }
-    __syncthreads();
-    if (tid == 0) sh.count = l.held;
-    __syncthreads();
+    if (l.sorted == k && l.held == k) {
+      l.thr_key = sh.cand[k - 1];
+      const f32 v = st_value((u32)(l.thr_key >> 32));
+      l.thr = v != v ? ROW_INF : v;
+#if ROW_F16
+      l.thr2 = row_x2h2(l.thr, l.thr);
+#endif
+    }
   }
-  if (n == 0) __syncthreads();
-  return true;
+  return l;
 }
 #endif
 
@@ -206,7 +241,6 @@ extern "C" __global__ void __launch_bounds__(ROW_THREADS, ROW_MIN_BLOCKS)
 __cluster_dims__(ROW_C, 1, 1)
 #endif
 acc_rows_stats(const __grid_constant__ Params p) {
-  __shared__ st_shared sh;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const i64 row = blockIdx.x / ROW_C;
   const int part = (int)(blockIdx.x % ROW_C);
@@ -220,8 +254,8 @@ acc_rows_stats(const __grid_constant__ Params p) {
   row_stat st = {-ROW_INF, 0.0f, 0.0f};
 #if ROW_TOPK
   st_list list;
-  int drained = b0, due = b0;            // tiles from `drained` on have blocks in the list; it is drained behind tile `due`
-  if (tid == 0) sh.count = sh.hot_count = 0;
+  int drained = b0, due = b0;            // blocks from `drained` on are not in the list of candidates yet; the next drain is behind tile `due`
+  if (tid == 0) sh.count = sh.hot_count[0] = sh.hot_count[1] = 0;
   __syncthreads();
 #endif
 
@@ -246,6 +280,61 @@ acc_rows_stats(const __grid_constant__ Params p) {
       row_unpack(cur[u], v);
       mb[u] = row_max_nan(row_max_nan(v[0], v[1]), row_max_nan(v[2], v[3]));
       mc = u == 0 ? mb[0] : row_max_nan(mc, mb[u]);
+    }
+#endif
+#if ROW_TOPK
+    if (t == b0) {
+      // The first tile sets the threshold, a key that at least k elements of the tile reach and few more.  Every warp
+      // answers for its share of the k: with T the largest 16-bit prefix that so many of its lanes' maxima reach, it
+      // takes all maxima above T and, lane by lane, as many at T as are missing; the least key among those (rounded
+      // down to the end of its block).
+      const int share = (k + ST_WARPS - 1) / ST_WARPS;
+      const u32 pre = mc == -ROW_INF ? 0u : (st_order(mc) >> 16);
+      u32 T = 0;
+#pragma unroll 1
+      for (u32 bit = 1u << 15; bit != 0; bit >>= 1)
+        if (__popc(__ballot_sync(ACC_FULL_MASK, pre >= (T | bit))) >= share) T |= bit;
+      u64 least = ST_NONE + 1;           // (fewer maxima than its share: no bound but -inf)
+      if (T != 0) {
+        const int above = __popc(__ballot_sync(ACC_FULL_MASK, pre > T));
+        const u32 ties = __ballot_sync(ACC_FULL_MASK, pre == T);
+        least = ~(u64)0;
+        if (pre == T && __popc(ties & ((1u << lane) - 1)) < share - above) {
+          int last = 0;
+#pragma unroll
+          for (int u = ROW_U - 1; u >= 0; --u)
+            if (st_block_max(mb[u]) == mc || mc != mc) last = span.first(t + u * ROW_THREADS + tid) + ROW_E - 1;
+          if (mc != mc) last = 0x7fffffff;
+          least = st_key(mc, last);
+        }
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) {
+          const u64 o = __shfl_xor_sync(ACC_FULL_MASK, least, d);
+          least = o < least ? o : least;
+        }
+      }
+      if (lane == 0) sh.key[warp] = least;
+      __syncthreads();
+      for (int w = 0; w < ST_WARPS; ++w) least = sh.key[w] < least ? sh.key[w] : least;
+      list.thr_key = least - 1;
+    }
+    // (later elements of the threshold's own value stand behind it: their indices are higher)
+    if (t == b0) {
+#pragma unroll
+      for (int u = 0; u < ROW_U; ++u) {
+        const int i = t + u * ROW_THREADS + tid;
+        st_push(list, cur[u], st_block_max(mb[u]), i, span.first(i));
+      }
+    } else if (!(mc <= list.thr) && !list.overflow) {
+#pragma unroll
+      for (int u = 0; u < ROW_U; ++u)
+        if (st_above(mb[u], list)) {
+          const int slot = atomicAdd(&sh.hot_count[list.phase], 1);
+          if (slot < ST_HOT) {
+            sh.hot[slot] = cur[u];
+            sh.hot_block[slot] = t + u * ROW_THREADS + tid;
+          }
+        }
     }
 #endif
     // statistics
@@ -287,79 +376,36 @@ acc_rows_stats(const __grid_constant__ Params p) {
     st.w += w0 + w1;
 
 #if ROW_TOPK
-    if (t == b0) {
-      // The first tile sets the threshold.  With T the largest 16-bit prefix that k threads' maxima reach, take all
-      // maxima above T and, thread by thread, as many at T as make k: the least key among them (each rounded down to
-      // the end of its block) is reached by k elements of the tile, and few more pass it.
-      const u32 pre = mc == -ROW_INF ? 0u : (st_order(mc) >> 16);
-      u32 T = 0;
-      for (int bit = 15; bit >= 0; --bit) {
-        const u32 trial = T | (1u << bit);
-        if (__syncthreads_count(pre >= trial) >= k) T = trial;
-      }
-      if (T != 0) {
-        const int above = __syncthreads_count(pre > T);
-        const u32 ties = __ballot_sync(ACC_FULL_MASK, pre == T);
-        if (lane == 0) sh.warp_count[warp] = __popc(ties);
-        __syncthreads();
-        int before = __popc(ties & ((1u << lane) - 1));
-        for (int w = 0; w < warp; ++w) before += sh.warp_count[w];
-        u64 least = ~(u64)0;
-        if (pre == T && before < k - above) {
-          int last = 0;
-#pragma unroll
-          for (int u = ROW_U - 1; u >= 0; --u)
-            if (st_order(st_block_max(mb[u])) == st_order(mc)) last = span.first(t + u * ROW_THREADS + tid) + ROW_E - 1;
-          least = st_key(mc, last);
-        }
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) {
-          const u64 o = __shfl_xor_sync(ACC_FULL_MASK, least, d);
-          least = o < least ? o : least;
-        }
-        if (lane == 0) sh.key[warp] = least;
-        __syncthreads();
-        for (int w = 0; w < ST_WARPS; ++w) least = sh.key[w] < least ? sh.key[w] : least;
-        if (least - 1 > list.thr_key) list.thr_key = least - 1;
-      }
-    }
-    // (later elements of the threshold's own value stand behind it: their indices are higher)
-    if (t == b0 ? mc != -ROW_INF : !(mc <= list.thr)) {
-#pragma unroll
-      for (int u = 0; u < ROW_U; ++u) {
-        const int i = t + u * ROW_THREADS + tid;
-        st_push(sh, list, cur[u], st_block_max(mb[u]), i, span.first(i));
-      }
-    }
     // The list is drained behind the first tile and whenever the part of the row seen since has doubled: each time
     // about k elements are expected above the old threshold.  Warps run on their own in between.
     if (t >= due || t + ST_TILE >= b1) {
-      if (!st_drain(sh, list, span, k)) {
-        // More blocks than the list holds (a row in rising order): once more over the same tiles, with the list
-        // drained as often as it may fill up.
-        const int end = min(t + ST_TILE, b1);
-        for (int s = drained; s < end; s += ST_HOT) {
-#pragma unroll 1
-          for (int u = 0; u < ST_HOT / ROW_THREADS; ++u) {
-            const int i = s + u * ROW_THREADS + tid;
-            if (i < end) {
-              const uint4 block = span.load(i);
-              f32 v[ROW_E], most;
-              row_unpack(block, v);
-              most = v[0];
-#pragma unroll
-              for (int e = 1; e < ROW_E; ++e) most = row_max_nan(most, v[e]);
-              st_push(sh, list, block, most, i, span.first(i));
-            }
-          }
-          st_drain(sh, list, span, k);
-        }
-      }
-      drained = t + ST_TILE;
-      due = drained + (drained - b0) - ST_TILE;
+      if (!list.overflow) list = st_drain(list, span.shift, k);
+      if (!list.overflow) drained = t + ST_TILE;
+      due = t + ST_TILE + (t - b0);
     }
 #endif
   }
+#if ROW_TOPK
+  if (list.overflow)
+    // More blocks came than the list holds (a row in rising order): once more over the tiles since, with the list
+    // drained as often as it may fill up.
+    for (int s = drained; s < b1; s += ST_HOT) {
+#pragma unroll 1
+      for (int u = 0; u < ST_HOT / ROW_THREADS; ++u) {
+        const int i = s + u * ROW_THREADS + tid;
+        if (i < b1) {
+          const uint4 block = span.load(i);
+          f32 v[ROW_E], most;
+          row_unpack(block, v);
+          most = v[0];
+#pragma unroll
+          for (int e = 1; e < ROW_E; ++e) most = row_max_nan(most, v[e]);
+          st_push(list, block, most, i, span.first(i));
+        }
+      }
+      list = st_drain(list, span.shift, k);
+    }
+#endif
 #if ROW_TOPK
   int held = list.held;                  // (sorted by the last drain)
   if (tid == 0) sh.kept = held;
@@ -382,26 +428,30 @@ acc_rows_stats(const __grid_constant__ Params p) {
   if (tid == 0) sh.cta = st;
   st_cluster_sync();
   if (part == 0) {
-    for (int r = 1; r < ROW_C; ++r) {
-      const u32 a = st_cluster_addr(&sh.cta, r);
-      row_stat o;
+    row_stat o[ROW_C];
+#pragma unroll
+    for (int r = 1; r < ROW_C; ++r)
       asm volatile("ld.shared::cluster.f32 %0, [%3];\n ld.shared::cluster.f32 %1, [%3 + 4];\n ld.shared::cluster.f32 %2, [%3 + 8];"
-                   : "=f"(o.m), "=f"(o.z), "=f"(o.w) : "r"(a));
-      st = st_join(st, o, c);
-    }
+                   : "=f"(o[r].m), "=f"(o[r].z), "=f"(o[r].w) : "r"(st_cluster_addr(&sh.cta, r)));
+#pragma unroll
+    for (int r = 1; r < ROW_C; ++r) st = st_join(st, o[r], c);
 #if ROW_TOPK
+    const int own = held;
+    int more[ROW_C];
+    u64 key[ROW_C];
+#pragma unroll
+    for (int r = 1; r < ROW_C; ++r)
+      asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(more[r]) : "r"(st_cluster_addr(&sh.kept, r)));
+#pragma unroll
+    for (int r = 1; r < ROW_C; ++r)      // (at most k <= 128 of them: one per thread)
+      if (tid < more[r]) asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(key[r]) : "r"(st_cluster_addr(&sh.cand[tid], r)));
+#pragma unroll
     for (int r = 1; r < ROW_C; ++r) {
-      int more;
-      asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(more) : "r"(st_cluster_addr(&sh.kept, r)));
-      if (tid < more) {                  // (at most k <= 128 of them: one per thread)
-        u64 key;
-        asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(key) : "r"(st_cluster_addr(&sh.cand[tid], r)));
-        sh.cand[held + tid] = key;
-      }
-      held += more;
+      if (tid < more[r]) sh.cand[held + tid] = key[r];
+      held += more[r];
     }
     __syncthreads();
-    held = st_compact(sh, held, k);
+    held = st_compact(own, held, k);
 #endif
   }
   st_cluster_sync();                     // nobody leaves while its shared memory is being read
