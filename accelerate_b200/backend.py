@@ -17,6 +17,7 @@ from . import language as L
 _HERE = os.path.dirname(os.path.abspath(__file__))
 _LIB_PATH = os.path.join(_HERE, "libaccb200.so")
 _lib = None
+_fast = None          # the compiled binding of the calls that every run makes (csrc/python/binding.cpp)
 
 ERRORS = {1: "parse", 2: "type", 3: "compile", 4: "cuda", 5: "bounds", 6: "unsupported", 7: "argument", 8: "timeout", 9: "arithmetic"}
 
@@ -32,7 +33,7 @@ class B200Error(RuntimeError):
 
 def lib():
     """The loaded C-ABI library; raises if it has not been built."""
-    global _lib
+    global _lib, _fast
     if _lib is None:
         if not os.path.exists(_LIB_PATH):
             raise B200Error(4, f"{_LIB_PATH} is missing: build it with `python -m accelerate_b200.build` (no CPU fallback exists)")
@@ -83,7 +84,14 @@ def lib():
         l.b200_compile_check.argtypes = [cp, ctypes.c_size_t, ctypes.c_char_p, ctypes.c_size_t]
         l.b200_kernel_source.argtypes = [cp, ctypes.c_size_t, ctypes.c_int, ctypes.c_char_p, ctypes.c_size_t]
         l.b200_program_lowered.argtypes = [cp, ctypes.c_size_t, ctypes.c_char_p, ctypes.c_size_t]
-        _lib = l
+        try:
+            from . import _binding
+        except ImportError as e:
+            raise B200Error(4, f"the compiled binding is missing ({e}): build it with `python -m accelerate_b200.build`") from e
+        address = lambda f: ctypes.cast(f, vp).value  # noqa: E731
+        _binding.setup(address(l.b200_array_wrap), address(l.b200_program_run), address(l.b200_array_info), address(l.b200_array_devptr),
+                       address(l.b200_array_free), address(l.b200_last_error), B200Error, tuple(L.SCALARS))
+        _lib, _fast = l, _binding
     return _lib
 
 
@@ -145,23 +153,26 @@ class DeviceArray:
     """A device-resident array (struct-of-arrays) owned by a context.  Whoever made it and knows its element type and
     shape passes both; otherwise the library is asked, once."""
 
-    def __init__(self, ctx, ident, elt=None, shape=None):
-        self.ctx, self.id = ctx, ident
-        if elt is not None and shape is not None:
-            self.elt, self.shape, self.leaf_types = elt, shape, _leaf_types(elt)
-            return
-        rank, leaves = ctypes.c_int(), ctypes.c_int()
-        for most_rank, most_leaves in ((8, 32), (1 << 10, 1 << 16)):
-            sh, types = (ctypes.c_int64 * most_rank)(), (ctypes.c_int32 * most_leaves)()
-            rc = lib().b200_array_info(ctx.h, ident, most_rank, ctypes.byref(rank), sh, most_leaves, ctypes.byref(leaves), types)
-            if rc == 0:
-                break
-        _check(rc)
-        self.shape = tuple(sh[:rank.value])
-        self.leaf_types = [L.SCALARS[k] for k in types[:leaves.value]]
-        self.elt = elt if elt is not None else (self.leaf_types[0] if leaves.value == 1 else tuple(self.leaf_types))
+    def __init__(self, ctx, ident, elt=None, shape=None, leaf_types=None, ptrs=None):
+        self.ctx, self.id, self._ptrs = ctx, ident, ptrs
+        if shape is not None and (elt is not None or leaf_types is not None):
+            self.shape = shape
+            self.leaf_types = leaf_types if leaf_types is not None else list(_leaf_types(elt))
+        else:
+            rank, leaves = ctypes.c_int(), ctypes.c_int()
+            for most_rank, most_leaves in ((8, 32), (1 << 10, 1 << 16)):
+                sh, types = (ctypes.c_int64 * most_rank)(), (ctypes.c_int32 * most_leaves)()
+                rc = lib().b200_array_info(ctx.h, ident, most_rank, ctypes.byref(rank), sh, most_leaves, ctypes.byref(leaves), types)
+                if rc == 0:
+                    break
+            _check(rc)
+            self.shape = tuple(sh[:rank.value])
+            self.leaf_types = [L.SCALARS[k] for k in types[:leaves.value]]
+        self.elt = elt if elt is not None else (self.leaf_types[0] if len(self.leaf_types) == 1 else tuple(self.leaf_types))
 
     def devptr(self, leaf=0):
+        if self._ptrs is not None and 0 <= leaf < len(self._ptrs):
+            return self._ptrs[leaf]
         p = ctypes.c_void_p()
         _check(lib().b200_array_devptr(self.ctx.h, self.id, leaf, ctypes.byref(p)))
         return p.value or 0
@@ -175,6 +186,7 @@ class DeviceArray:
     def adopt_host(self, leaves):
         """Lazy upload: the host arrays are copied when the array is first used on the device;
         they are kept alive by this object until then."""
+        self._ptrs = None                # (the library copies the payload when it is next asked for the pointer)
         self._adopted = [np.ascontiguousarray(a) for a in leaves]
         for k, a in enumerate(self._adopted):
             _check(lib().b200_array_adopt_host(self.ctx.h, self.id, k, a.ctypes.data, a.nbytes))
@@ -202,9 +214,9 @@ class DeviceArray:
         return out[0] if L.is_scalar(self.elt) else tuple(out)
 
     def free(self):
-        if self.id is not None and self.ctx.h:
-            lib().b200_array_free(self.ctx.h, self.id)
-            self.id = None
+        if self.id is not None and self.ctx.handle:
+            _fast.free(self.ctx.handle, self.id)
+            self.id = self._ptrs = None
 
     def __del__(self):
         try:
@@ -219,6 +231,7 @@ class Context:
     def __init__(self, device=0):
         self.h = ctypes.c_void_p()
         _check(lib().b200_ctx_create(device, 0, ctypes.byref(self.h)))
+        self.handle = self.h.value           # the same as a number; 0 once the context is closed
         self.device = device
         self._programs = {}
         self._inflight = []          # views with an asynchronous download under way (kept alive until sync)
@@ -229,6 +242,7 @@ class Context:
             for p in self._programs.values():
                 lib().b200_program_free(p)
             self._programs = {}
+            self.handle = 0
             lib().b200_ctx_destroy(self.h)
             self.h = ctypes.c_void_p()
 
@@ -279,11 +293,10 @@ class Context:
 
     def wrap(self, elt, shape, ptrs):
         """Adopt caller-owned device memory (one pointer per leaf)."""
-        ident = ctypes.c_uint64()
-        sh = (ctypes.c_int64 * max(1, len(shape)))(*shape)
-        arr = (ctypes.c_void_p * len(ptrs))(*ptrs)
-        _check(lib().b200_array_wrap(self.h, _elt_text(elt), len(shape), sh, arr, ctypes.byref(ident)))
-        return DeviceArray(self, ident.value, elt, tuple(map(int, shape)))
+        if len(ptrs) != len(_leaf_types(elt)):
+            raise ValueError("one pointer per scalar leaf of the element type")
+        shape = tuple(map(int, shape))
+        return DeviceArray(self, _fast.wrap(self.handle, _elt_text(elt), shape, ptrs), elt, shape)
 
     # programs ---------------------------------------------------------------
     def load(self, text):
@@ -298,10 +311,8 @@ class Context:
     def execute(self, text, inputs, n_out):
         """Run program ``text`` on device arrays; returns device arrays."""
         p = self.load(text)
-        ins = (ctypes.c_uint64 * max(1, len(inputs)))(*[a.id for a in inputs])
-        outs = (ctypes.c_uint64 * max(1, n_out))()
-        _check(lib().b200_program_run(p, ins, len(inputs), outs, n_out))
-        return [DeviceArray(self, outs[k]) for k in range(n_out)]
+        return [DeviceArray(self, ident, None, shape, types, ptrs)
+                for ident, shape, types, ptrs in _fast.execute(self.handle, p.value, [a.id for a in inputs], n_out)]
 
     def run_rows(self, text, inputs, out, row_lo, row_hi):
         """Rows [row_lo, row_hi) of a one-stencil-node program's result, into the existing array ``out``."""

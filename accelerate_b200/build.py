@@ -4,7 +4,8 @@
 NVRTC kernel cache, runtime, C ABI) and the text of the hand-written sm_100a
 skeletons (``csrc/skeletons/*.cuh``), which NVRTC compiles together with the
 generated scalar code at run time.  Ahead-of-time CUDA sources (``csrc/*.cu``)
-are compiled by nvcc for sm_100a and linked in.
+are compiled by nvcc for sm_100a and linked in.  ``_binding.so`` is the CPython module that
+makes a run's calls.
 """
 from __future__ import annotations
 
@@ -12,10 +13,12 @@ import glob
 import os
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "libaccb200.so")
+BINDING = os.path.join(HERE, "_binding.so")
 CUDA = os.environ.get("CUDA_HOME", "/usr/local/cuda")
 NVCC_ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
@@ -52,7 +55,19 @@ def _newer(target, sources):
     return any(os.path.getmtime(s) > t for s in sources)
 
 
+def _build_binding(force, verbose):
+    """The CPython module for the calls that every run makes (csrc/python/binding.cpp)."""
+    src = os.path.join(CSRC, "python", "binding.cpp")
+    if not force and not _newer(BINDING, [src, os.path.abspath(__file__)]):
+        return
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", f"-I{sysconfig.get_paths()['include']}", src, "-o", BINDING]
+    if verbose:
+        print(" ".join(cmd))
+    subprocess.check_call(cmd)
+
+
 def build(force=False, verbose=False):
+    _build_binding(force, verbose)
     _embed_skeletons()
     cpps = sorted(glob.glob(os.path.join(CSRC, "*.cpp")))
     cus = sorted(glob.glob(os.path.join(CSRC, "*.cu")))

@@ -1,0 +1,183 @@
+// The calls that every run of a program makes from Python, without ctypes: wrap, execute, free.  A call through
+// ctypes costs about a microsecond and a half, and a run makes a dozen of them; a small kernel takes two.  Everything
+// else of the C ABI goes through ctypes (backend.py), which also hands over the entry points' addresses.
+#define PY_SSIZE_T_CLEAN
+#include <Python.h>
+
+#include <cstdint>
+#include <vector>
+
+namespace {
+
+int (*f_wrap)(void*, const char*, int, const int64_t*, void* const*, uint64_t*);
+int (*f_run)(void*, const uint64_t*, int, uint64_t*, int);
+int (*f_info)(void*, uint64_t, int, int*, int64_t*, int, int*, int32_t*);
+int (*f_devptr)(void*, uint64_t, int, void**);
+int (*f_free)(void*, uint64_t);
+const char* (*f_error)();
+PyObject* error_class;      // B200Error(code, message)
+PyObject* type_names;       // scalar types in the library's order
+
+PyObject* fail(int rc) {
+  PyObject* args = Py_BuildValue("(is)", rc, f_error());
+  if (args) {
+    PyErr_SetObject(error_class, args);
+    Py_DECREF(args);
+  }
+  return nullptr;
+}
+bool to_u64(PyObject* o, uint64_t* v) {
+  *v = PyLong_AsUnsignedLongLong(o);
+  return !(*v == (uint64_t)-1 && PyErr_Occurred());
+}
+// rank, extents and leaves of an array as (shape, leaf types)
+constexpr int kRank = 1024, kLeaves = 1 << 16;
+bool describe(void* ctx, uint64_t id, int* rank, std::vector<int64_t>& shape, int* leaves, std::vector<int32_t>& types, int* rc) {
+  shape.resize(8);
+  types.resize(32);
+  *rc = f_info(ctx, id, 8, rank, shape.data(), 32, leaves, types.data());
+  if (*rc) {
+    shape.resize(kRank);
+    types.resize(kLeaves);
+    *rc = f_info(ctx, id, kRank, rank, shape.data(), kLeaves, leaves, types.data());
+  }
+  return *rc == 0;
+}
+
+// setup(wrap, run, info, devptr, free, last_error, error class, type names)
+PyObject* setup(PyObject*, PyObject* args) {
+  unsigned long long a[6];
+  PyObject *e, *t;
+  if (!PyArg_ParseTuple(args, "KKKKKKOO!", &a[0], &a[1], &a[2], &a[3], &a[4], &a[5], &e, &PyTuple_Type, &t)) return nullptr;
+  f_wrap = (decltype(f_wrap))a[0];
+  f_run = (decltype(f_run))a[1];
+  f_info = (decltype(f_info))a[2];
+  f_devptr = (decltype(f_devptr))a[3];
+  f_free = (decltype(f_free))a[4];
+  f_error = (decltype(f_error))a[5];
+  Py_INCREF(e);
+  Py_INCREF(t);
+  error_class = e;
+  type_names = t;
+  Py_RETURN_NONE;
+}
+
+// wrap(ctx, element type, shape, pointers) -> id
+PyObject* wrap(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  uint64_t ctx;
+  if (n != 4 || !f_wrap) return PyErr_Format(PyExc_TypeError, "wrap(ctx, elt, shape, ptrs)");
+  if (!to_u64(args[0], &ctx)) return nullptr;
+  const char* elt = PyBytes_AsString(args[1]);
+  if (!elt) return nullptr;
+  PyObject *shape = PySequence_Fast(args[2], "a shape is a sequence"), *ptrs = nullptr;
+  if (shape) ptrs = PySequence_Fast(args[3], "one pointer per leaf");
+  PyObject* r = nullptr;
+  if (ptrs) {
+    std::vector<int64_t> sh;
+    std::vector<void*> p;
+    for (Py_ssize_t i = 0; i < PySequence_Fast_GET_SIZE(shape); ++i) sh.push_back(PyLong_AsLongLong(PySequence_Fast_GET_ITEM(shape, i)));
+    for (Py_ssize_t i = 0; i < PySequence_Fast_GET_SIZE(ptrs) && !PyErr_Occurred(); ++i) {
+      PyObject* q = PySequence_Fast_GET_ITEM(ptrs, i);
+      PyObject* ix = q == Py_None ? nullptr : PyNumber_Index(q);
+      p.push_back(ix ? PyLong_AsVoidPtr(ix) : nullptr);
+      Py_XDECREF(ix);
+    }
+    if (!PyErr_Occurred()) {
+      uint64_t id = 0;
+      int rc;
+      p.push_back(nullptr);
+      sh.push_back(0);
+      Py_BEGIN_ALLOW_THREADS
+      rc = f_wrap((void*)ctx, elt, (int)sh.size() - 1, sh.data(), p.data(), &id);
+      Py_END_ALLOW_THREADS
+      r = rc ? fail(rc) : PyLong_FromUnsignedLongLong(id);
+    }
+  }
+  Py_XDECREF(shape);
+  Py_XDECREF(ptrs);
+  return r;
+}
+
+// execute(ctx, program, input ids, number of results) -> [(id, shape, leaf types, pointers)]
+PyObject* execute(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  uint64_t ctx, prog;
+  if (n != 4 || !f_run) return PyErr_Format(PyExc_TypeError, "execute(ctx, program, ids, results)");
+  if (!to_u64(args[0], &ctx) || !to_u64(args[1], &prog)) return nullptr;
+  const long n_out = PyLong_AsLong(args[3]);
+  if (n_out == -1 && PyErr_Occurred()) return nullptr;
+  if (n_out < 0 || n_out > 1 << 20) return PyErr_Format(PyExc_ValueError, "bad number of results");
+  PyObject* seq = PySequence_Fast(args[2], "ids are a sequence");
+  if (!seq) return nullptr;
+  std::vector<uint64_t> ins((size_t)PySequence_Fast_GET_SIZE(seq) + 1), outs((size_t)n_out + 1);
+  const int n_in = (int)ins.size() - 1;
+  bool ok = true;
+  for (int i = 0; ok && i < n_in; ++i) ok = to_u64(PySequence_Fast_GET_ITEM(seq, i), &ins[i]);
+  Py_DECREF(seq);
+  if (!ok) return nullptr;
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = f_run((void*)prog, ins.data(), n_in, outs.data(), (int)n_out);
+  Py_END_ALLOW_THREADS
+  if (rc) return fail(rc);
+  // (on any failure from here on the results are released again: nobody else knows their ids)
+  PyObject* list = PyList_New(n_out);
+  std::vector<int64_t> shape;
+  std::vector<int32_t> types;
+  for (long k = 0; list && k < n_out; ++k) {
+    int rank = 0, leaves = 0;
+    std::vector<void*> ptr;
+    bool good = describe((void*)ctx, outs[k], &rank, shape, &leaves, types, &rc);
+    for (int l = 0; good && l < leaves; ++l) {
+      ptr.push_back(nullptr);
+      good = (rc = f_devptr((void*)ctx, outs[k], l, &ptr.back())) == 0;
+    }
+    PyObject* item = nullptr;
+    if (!good) {
+      fail(rc);
+    } else {
+      PyObject *sh = PyTuple_New(rank), *ty = PyList_New(leaves), *pt = PyTuple_New(leaves);
+      for (int d = 0; sh && d < rank; ++d) PyTuple_SET_ITEM(sh, d, PyLong_FromLongLong(shape[d]));
+      for (int l = 0; ty && pt && l < leaves; ++l) {
+        PyObject* name = PyTuple_GetItem(type_names, types[l]);
+        Py_XINCREF(name);
+        PyList_SET_ITEM(ty, l, name);
+        PyTuple_SET_ITEM(pt, l, PyLong_FromVoidPtr(ptr[l]));
+      }
+      if (sh && ty && pt && !PyErr_Occurred()) item = Py_BuildValue("(KOOO)", (unsigned long long)outs[k], sh, ty, pt);
+      Py_XDECREF(sh);
+      Py_XDECREF(ty);
+      Py_XDECREF(pt);
+    }
+    if (!item) {
+      Py_CLEAR(list);
+      break;
+    }
+    PyList_SET_ITEM(list, k, item);
+  }
+  if (!list)
+    for (long k = 0; k < n_out; ++k) f_free((void*)ctx, outs[k]);
+  return list;
+}
+
+// free(ctx, id): as b200_array_free; the result is its status
+PyObject* free_(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  uint64_t ctx, id;
+  if (n != 2 || !f_free) return PyErr_Format(PyExc_TypeError, "free(ctx, id)");
+  if (!to_u64(args[0], &ctx) || !to_u64(args[1], &id)) return nullptr;
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = f_free((void*)ctx, id);
+  Py_END_ALLOW_THREADS
+  return PyLong_FromLong(rc);
+}
+
+PyMethodDef methods[] = {{"setup", setup, METH_VARARGS, nullptr},
+                         {"wrap", (PyCFunction)(void (*)(void))wrap, METH_FASTCALL, nullptr},
+                         {"execute", (PyCFunction)(void (*)(void))execute, METH_FASTCALL, nullptr},
+                         {"free", (PyCFunction)(void (*)(void))free_, METH_FASTCALL, nullptr},
+                         {nullptr, nullptr, 0, nullptr}};
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_binding", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
+
+}  // namespace
+
+PyMODINIT_FUNC PyInit__binding() { return PyModule_Create(&module); }

@@ -141,11 +141,13 @@ constexpr int kThreads = 256, kStatsThreads = 128;
 Variant stats_variant(int ctas) { return {{"ROW_THREADS", str(kStatsThreads)}, {"ROW_U", "8"}, {"ROW_MIN_BLOCKS", "7"}, {"ROW_C", str(ctas)}}; }
 Variant distill_grad_variant(int ctas) { return {{"ROW_THREADS", str(kThreads)}, {"ROW_U", "4"}, {"ROW_MIN_BLOCKS", "4"}, {"ROW_C", str(ctas)}}; }
 
-// CTAs that share a row: enough to give every SM several, as long as each has a tile of its own
-int ctas_per_row(int64_t rows, int64_t n, int elt_bytes, int sms, int most) {
+// CTAs that share a row: enough to give every SM `several`, as long as each has a tile of its own.  The statistics
+// take 4 (500 rows of 50257 Floats, k = 5: 2 CTAs per row 28.7 us, 4 CTAs 42 us: every CTA finds a threshold of its
+// own), the gradient 8 (333 rows of 50257: 31.6 us with 8, 35.0 with 4).
+int ctas_per_row(int64_t rows, int64_t n, int elt_bytes, int sms, int several, int most) {
   const int64_t tiles = (n * elt_bytes + 16 * kThreads * 4 - 1) / (16 * kThreads * 4);
   int c = 1;
-  while (c < most && rows * c < 8 * (int64_t)sms && 2 * c <= tiles) c *= 2;
+  while (c < most && rows * c < several * (int64_t)sms && 2 * c <= tiles) c *= 2;
   return c;
 }
 
@@ -274,7 +276,7 @@ void Program::exec_foreign(const Node& n, Env& env) {
       env[n.outs[0]] = stats;
       env[n.outs[1]] = top;
       if (rows == 0) break;
-      const int ctas = ctas_per_row(rows, cols, elt_bytes, c.sm_count, 8);
+      const int ctas = ctas_per_row(rows, cols, elt_bytes, c.sm_count, 4, 8);
       const size_t smem = stats_smem(k > 0);
       CompiledKernel& ker = shape_kernel(c, st, (uint64_t)ctas, "rows_stats", [&] { return stats_variant(ctas); }, "acc_rows_stats", kStatsThreads, smem);
       launch(c, ker, rows * ctas, kStatsThreads, smem,
@@ -293,7 +295,7 @@ void Program::exec_foreign(const Node& n, Env& env) {
         env[n.outs[0]] = loss;
         env[n.outs[1]] = lse;
         if (rows == 0) break;
-        const int ctas = ctas_per_row(rows, cols, elt_bytes, c.sm_count, 8);
+        const int ctas = ctas_per_row(rows, cols, elt_bytes, c.sm_count, 4, 8);
         const size_t smem = stats_smem(false);
         CompiledKernel& ker = shape_kernel(c, st, (uint64_t)ctas, "rows_stats", [&] { return stats_variant(ctas); }, "acc_rows_stats", kStatsThreads, smem);
         launch(c, ker, rows * ctas, kStatsThreads, smem,
@@ -305,7 +307,7 @@ void Program::exec_foreign(const Node& n, Env& env) {
         DevArrayP dx = c.new_array(n.out_info[0].elt, x.shape);
         env[n.outs[0]] = dx;
         if (rows == 0 || cols == 0) break;
-        const int ctas = ctas_per_row(rows, cols, elt_bytes, c.sm_count, 16);
+        const int ctas = ctas_per_row(rows, cols, elt_bytes, c.sm_count, 8, 16);
         CompiledKernel& ker = shape_kernel(c, st, (uint64_t)ctas, "rows_distill_grad", [&] { return distill_grad_variant(ctas); }, "acc_rows_distill_grad", kThreads, 0);
         launch(c, ker, rows * ctas, kThreads, 0,
                {ptr_of(x), ptr_of(*a[0]), ptr_of(*a[1]), ptr_of(*a[3]), ptr_of(*a[4]), ptr_of(*dx), (uint64_t)rows, (uint64_t)cols, (uint64_t)k,

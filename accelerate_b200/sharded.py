@@ -99,7 +99,8 @@ class GpuExecutor:
         exchange steps go through ``torch.distributed`` on views of the device arrays."""
         from . import backend
         self.backend, self.ctx, self.group = backend, ctx, group
-        self.stream = torch.cuda.ExternalStream(ctx.stream(), device=torch.device("cuda", ctx.device))
+        self.device = torch.device("cuda", ctx.device)
+        self.stream = torch.cuda.ExternalStream(ctx.stream(), device=self.device)
         self._progs = ProgramCache()
 
     @classmethod
@@ -143,7 +144,7 @@ class GpuExecutor:
         if 0 in a.shape:
             dt = np.dtype(L.NP_OF[a.leaf_types[leaf]])
             return torch.empty(a.shape, dtype=torch.from_numpy(np.empty(0, dt)).dtype, device=self.stream.device)
-        t = torch.as_tensor(_View(a, leaf), device=self.stream.device)
+        t = torch.as_tensor(_View(a, leaf), device=self.device)
         t._keepalive = a
         return t
 
