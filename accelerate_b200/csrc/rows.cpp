@@ -155,10 +155,15 @@ int ctas_per_row(int64_t rows, int64_t n, int elt_bytes, int sms, int several, i
 struct NormShape {
   int ve, warps, u, threads;
   bool whole;              // the row fits the registers
+  int stages = 0;          // gradients: rows in flight through shared memory
+  bool keep = true;        // gradients: a row's blocks stay in registers
   Variant variant() const {
-    return {{"ROW_THREADS", str(threads)}, {"NORM_VE", str(ve)}, {"NORM_WARPS", str(warps)}, {"NORM_U", str(u)}, {"NORM_LONG", whole ? "0" : "1"}};
+    return {{"ROW_THREADS", str(threads)}, {"NORM_VE", str(ve)},         {"NORM_WARPS", str(warps)},         {"NORM_U", str(u)},
+            {"NORM_LONG", whole ? "0" : "1"}, {"NORM_STAGES", str(stages)}, {"NORM_KEEP", keep ? "1" : "0"}};
   }
-  uint64_t key() const { return (uint64_t)ve << 40 | (uint64_t)warps << 32 | (uint64_t)u << 16 | (uint64_t)(threads / 32) << 8 | (whole ? 1 : 0); }
+  uint64_t key() const {
+    return (uint64_t)ve << 40 | (uint64_t)warps << 32 | (uint64_t)u << 16 | (uint64_t)(threads / 32) << 8 | (uint64_t)stages << 4 | (keep ? 2 : 0) | (whole ? 1 : 0);
+  }
   int rows() const { return threads / 32 / warps; }
 };
 // the next size of the list 1 2 3 4 6 8 12 16 ...: few kernels for all lengths
@@ -186,7 +191,40 @@ NormShape norm_shape(int64_t n, int ve, int most_elems, int most_warps, int64_t 
   return s;
 }
 constexpr int kNormElems = 32, kNormWarps = 32;          // forward: elements per thread, warps per row
-constexpr int kNormGradElems = 16, kNormGradWarps = 16;
+NormShape norm_forward_shape(int64_t n, int ve, int64_t rows, int sms) {
+  const NormShape s = norm_shape(n, ve, ve == 1 ? 8 : 32, 8, rows, sms);
+  return s.whole ? s : norm_shape(n, ve, kNormElems, kNormWarps, rows, sms);
+}
+constexpr int kNormGradElems = 16, kNormGradWarps = 16;  // gradients; twice the elements where they pass through shared memory
+// Shared memory per CTA for rows in flight: two CTAs of 256 threads per SM, or one of 512
+constexpr int64_t kRingBytes = 104 << 10, kRingBytesAlone = 208 << 10;
+NormShape norm_grad_shape(int64_t n, int ve, int64_t rows, int sms) {
+  if (ve == 1) {
+    // (one element per access: eight per lane leave the registers for three CTAs per SM)
+    const NormShape s = norm_shape(n, ve, kNormGradElems / 2, kNormGradWarps, rows, sms);
+    return s.whole ? s : norm_shape(n, ve, kNormGradElems, kNormGradWarps, rows, sms);
+  }
+  NormShape s = norm_shape(n, ve, kNormGradElems, kNormGradWarps, rows, sms);
+  int64_t rest = 0;
+  if (!s.whole) {
+    s = norm_shape(n, ve, 2 * kNormGradElems, kNormGradWarps, rows, sms);
+    if (!s.whole) return s;
+    s.keep = false;
+    rest = 4LL * s.u * s.threads * ve;       // gamma, for any length that comes to this shape
+  }
+  const int64_t stage = 2LL * 16 * s.u * s.threads, room = (s.threads > kThreads ? kRingBytesAlone : kRingBytes) - rest;
+  s.stages = (int)std::min<int64_t>(4, room / stage);
+  if (s.stages < 2) {
+    NormShape reread = {ve, 16, 1, 512, false};
+    return reread;
+  }
+  return s;
+}
+size_t norm_grad_smem(const NormShape& s, int64_t n) {
+  if (!s.whole) return 0;
+  const size_t ring = 2u * 16 * s.u * s.threads * s.stages + (s.keep ? 0 : 4u * s.u * s.threads * s.ve), sums = s.rows() > 1 ? (size_t)n * 8 : 0;
+  return std::max(ring, sums);
+}
 
 }  // namespace
 
@@ -201,13 +239,13 @@ std::vector<std::pair<std::string, Variant>> foreign_variants(const Node& n) {
     case F_DISTILL_GRAD: v.push_back({"rows_distill_grad", distill_grad_variant(1)}); break;
     case F_LAYER_NORM:
       for (int64_t len : {1024, 4096, 1 << 20})
-        for (int w : {ve, 1}) v.push_back({"rows_norm", norm_shape(len, w, kNormElems, kNormWarps, 1 << 20, 148).variant()});
+        for (int w : {ve, 1}) v.push_back({"rows_norm", norm_forward_shape(len, w, 1 << 20, 148).variant()});
       break;
     case F_LAYER_NORM_GRAD:
-      for (int64_t len : {1024, 4096, 1 << 20})
-        for (int w : {ve, 1}) v.push_back({"rows_norm_grad", with(norm_shape(len, w, kNormGradElems, kNormGradWarps, 1 << 20, 148).variant(), "")});
-      v.push_back({"rows_norm_grad", with(norm_shape(1, 1, 1, 1, 1, 1).variant(), "NORM_SUMS")});
-      v.push_back({"rows_norm_grad", with(norm_shape(1, 1, 1, 1, 1, 1).variant(), "NORM_COLS")});
+      for (int64_t len : {1024, 4096, 12000, 1 << 20})
+        for (int w : {ve, 1}) v.push_back({"rows_norm_grad", with(norm_grad_shape(len, w, 1 << 20, 148).variant(), "")});
+      v.push_back({"rows_norm_grad", with(NormShape{1, 1, 1, 1024, true}.variant(), "NORM_SUMS")});
+      v.push_back({"rows_norm_grad", with(NormShape{1, 1, 1, kThreads, true}.variant(), "NORM_COLS")});
       break;
     case F_NONE: break;
   }
@@ -322,7 +360,7 @@ void Program::exec_foreign(const Node& n, Env& env) {
       env[n.outs[1]] = stats;
       if (rows == 0) break;
       const bool wide = x.aligned16() && y->aligned16() && a[0]->aligned16() && a[1]->aligned16() && cols * elt_bytes % 16 == 0;
-      const NormShape s = norm_shape(cols, wide ? 16 / elt_bytes : 1, kNormElems, kNormWarps, rows, c.sm_count);
+      const NormShape s = norm_forward_shape(cols, wide ? 16 / elt_bytes : 1, rows, c.sm_count);
       CompiledKernel& ker = shape_kernel(c, st, s.key(), "rows_norm", [&] { return s.variant(); }, "acc_rows_norm", s.threads, 0);
       launch(c, ker, (rows + s.rows() - 1) / s.rows(), s.threads, 0,
              {ptr_of(x), ptr_of(*a[0]), ptr_of(*a[1]), ptr_of(*y), ptr_of(*stats, 0), ptr_of(*stats, 1), (uint64_t)rows, (uint64_t)cols, float_bits(n.consts[0])});
@@ -338,19 +376,21 @@ void Program::exec_foreign(const Node& n, Env& env) {
       env[n.outs[2]] = dbeta;
       if (cols == 0) break;
       const bool wide = x.aligned16() && dx->aligned16() && a[3]->aligned16() && a[0]->aligned16() && cols * elt_bytes % 16 == 0;
-      const NormShape s = norm_shape(cols, wide ? 16 / elt_bytes : 1, kNormGradElems, kNormGradWarps, rows, c.sm_count);
+      const NormShape s = norm_grad_shape(cols, wide ? 16 / elt_bytes : 1, rows, c.sm_count);
       // (one source for three kernels: which of them it compiles to)
       auto which = [&](bool sums, bool cols_) {
         return [&, sums, cols_] {
-          Variant v = sums || cols_ ? norm_shape(1, 1, 1, 1, 1, 1).variant() : s.variant();
+          Variant v = sums || cols_ ? NormShape{1, 1, 1, sums ? 1024 : kThreads, true}.variant() : s.variant();
           v["NORM_SUMS"] = sums ? "1" : "0";
           v["NORM_COLS"] = cols_ ? "1" : "0";
           return v;
         };
       };
-      const size_t smem = s.whole && s.rows() > 1 ? (size_t)cols * 8 : 0;
+      const size_t smem = norm_grad_smem(s, cols);
       CompiledKernel& ker = shape_kernel(c, st, s.key(), "rows_norm_grad", which(false, false), "acc_rows_norm_grad", s.threads, smem);
-      const int64_t grid = std::min<int64_t>((rows + s.rows() - 1) / s.rows(), (int64_t)c.sm_count * ker.max_blocks_per_sm);
+      // as many CTAs as fit at once, and few enough for four trips each: a CTA costs a line of partial sums
+      const int64_t groups = (rows + s.rows() - 1) / s.rows();
+      const int64_t grid = std::min(groups, std::min<int64_t>((int64_t)c.sm_count * ker.max_blocks_per_sm, std::max<int64_t>(c.sm_count, groups / 4)));
       // lines of partial sums: one per CTA; for long rows one per `chunk` rows
       const int64_t tiles = (cols + 31) / 32;
       int64_t lines = grid, chunk = 0;
@@ -366,8 +406,8 @@ void Program::exec_foreign(const Node& n, Env& env) {
         CompiledKernel& kc = shape_kernel(c, st, 1, "rows_norm_grad", which(false, true), "acc_rows_norm_cols", kThreads, 0);
         launch(c, kc, lines * tiles, kThreads, 0, params);
       }
-      CompiledKernel& ks = shape_kernel(c, st, 2, "rows_norm_grad", which(true, false), "acc_rows_norm_sums", kThreads, 0);
-      launch(c, ks, tiles, kThreads, 0, params);
+      CompiledKernel& ks = shape_kernel(c, st, 2, "rows_norm_grad", which(true, false), "acc_rows_norm_sums", 1024, 0);
+      launch(c, ks, tiles, 1024, 0, params);
       break;
     }
     case F_NONE: break;

@@ -4,10 +4,20 @@
 // the same columns of every row, so that the sums over rows stay in its registers.  At the end the CTA's sums go to
 // `partial` (one line of 2 n Floats per CTA) and acc_rows_norm_sums adds the lines in their order: the same
 // numbers every time, whatever order the CTAs ran in.
-// NORM_LONG: rows longer than the registers hold; dx alone (three reads of the row), the sums over rows by
-// acc_rows_norm_cols.
+//
+//   NORM_STAGES  rows of x and dy on their way while one is worked on: every lane copies its own 16-byte blocks to
+//                shared memory (cp.async) and reads them back itself, so the ring needs no barrier and no flag.  0: rows
+//                that do not start on 16-byte boundaries are loaded directly.
+//   NORM_KEEP    1: a row's blocks and gamma stay in registers between the two passes (up to 16 elements per lane);
+//                0: gamma lies in shared memory and the blocks are read from the ring twice (32 elements per lane,
+//                whose sums alone take 64 registers)
+//   NORM_LONG    rows longer than that: dx alone (x and dy read twice), the sums over rows by acc_rows_norm_cols
 
 struct Params { i64 x, gamma, mean, rstd, dy, dx, partial, dgamma, dbeta, rows, n, lines, chunk; };
+
+extern __shared__ uint4 norm_memory[];
+// gamma in registers where they suffice
+#define NORM_GAMMA_REGS (NORM_KEEP && (NORM_STAGES > 0 || NORM_U * NORM_VE <= 8))
 
 #if NORM_SUMS
 // Lines of partial sums -> dgamma, dbeta.  32 columns per CTA, the warps take lines in turn.
@@ -65,7 +75,7 @@ extern "C" __global__ void __launch_bounds__(ROW_THREADS) acc_rows_norm_cols(con
   }
 }
 #else
-extern "C" __global__ void __launch_bounds__(ROW_THREADS) acc_rows_norm_grad(const __grid_constant__ Params p) {
+extern "C" __global__ void __launch_bounds__(ROW_THREADS, ROW_THREADS > 256 ? 1 : 2) acc_rows_norm_grad(const __grid_constant__ Params p) {
 #if NORM_WARPS > 1
   __shared__ f32 red[2][ROW_THREADS / 32][2];
 #else
@@ -112,73 +122,137 @@ extern "C" __global__ void __launch_bounds__(ROW_THREADS) acc_rows_norm_grad(con
   f32 sg[NORM_U * NORM_VE], sb[NORM_U * NORM_VE];
 #pragma unroll
   for (int i = 0; i < NORM_U * NORM_VE; ++i) sg[i] = sb[i] = 0.0f;
-  norm_x bx[NORM_U], bd[NORM_U];
   i64 row = (i64)blockIdx.x * NORM_ROWS + sub;
   const i64 stride = (i64)gridDim.x * NORM_ROWS;
-  f32 mean = 0.0f, rstd = 0.0f;
+#if NORM_STAGES
+  // the ring: [stage][x, dy][access][thread], behind it gamma
+  uint4* const mine = norm_memory + threadIdx.x;
+  constexpr int PLANE = NORM_U * ROW_THREADS;
+  auto fetch = [&](i64 r, int stage) {
+    if (r < p.rows) {
+      const row_t* x = reinterpret_cast<const row_t*>(p.x) + r * p.n;
+      const row_t* dy = reinterpret_cast<const row_t*>(p.dy) + r * p.n;
+#pragma unroll
+      for (int u = 0; u < NORM_U; ++u) {
+        const int j = u * STEP + g * NORM_VE;
+        if (j < n) {
+          norm_copy(mine + (2 * stage) * PLANE + u * ROW_THREADS, x + j);
+          norm_copy(mine + (2 * stage + 1) * PLANE + u * ROW_THREADS, dy + j);
+        }
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int s = 0; s < NORM_STAGES - 1; ++s) fetch(row + s * stride, s);
+  int stage = 0;
+#endif
+#if !NORM_KEEP
+  f32* const gs = reinterpret_cast<f32*>(norm_memory + 2 * NORM_STAGES * PLANE);
+  for (int j = threadIdx.x; j < n; j += ROW_THREADS) gs[j] = row_wide(gamma[j]);
+  __syncthreads();
+#elif NORM_GAMMA_REGS
+  f32 gr[NORM_U][NORM_VE];
+#pragma unroll
+  for (int u = 0; u < NORM_U; ++u) {
+    const int j = u * STEP + g * NORM_VE;
+    if (j < n) norm_params(gamma + j, gr[u]);
+  }
+#endif
+  f32 mean = 0.0f, rstd = 0.0f, mean_next = 0.0f, rstd_next = 0.0f;
+  if (row < p.rows) {
+    mean_next = reinterpret_cast<const f32*>(p.mean)[row];
+    rstd_next = reinterpret_cast<const f32*>(p.rstd)[row];
+  }
   int slot = 0;
   // (a CTA's groups make the same number of trips: they share the barriers)
   for (i64 first = (i64)blockIdx.x * NORM_ROWS; first < p.rows; first += stride, row += stride) {
     const bool there = row < p.rows;
-    if (there) {
-      const row_t* x = reinterpret_cast<const row_t*>(p.x) + row * p.n;
-      const row_t* dy = reinterpret_cast<const row_t*>(p.dy) + row * p.n;
-#pragma unroll
-      for (int u = 0; u < NORM_U; ++u) {
-        const int j = u * STEP + g * NORM_VE;
-        if (j < n) {
-          bx[u] = norm_load(x + j);
-          bd[u] = norm_load(dy + j);
-        }
-      }
-      mean = reinterpret_cast<const f32*>(p.mean)[row];
-      rstd = reinterpret_cast<const f32*>(p.rstd)[row];
+    mean = mean_next;
+    rstd = rstd_next;
+    if (row + stride < p.rows) {
+      mean_next = reinterpret_cast<const f32*>(p.mean)[row + stride];
+      rstd_next = reinterpret_cast<const f32*>(p.rstd)[row + stride];
     }
+#if NORM_STAGES
+    // (the stage fetched into now was read in the trip before, by this thread)
+    fetch(row + (NORM_STAGES - 1) * stride, (stage + NORM_STAGES - 1) % NORM_STAGES);
+    asm volatile("cp.async.wait_group %0;" ::"n"(NORM_STAGES - 1) : "memory");
+    const uint4* const bx = mine + (2 * stage) * PLANE;
+    const uint4* const bd = mine + (2 * stage + 1) * PLANE;
+    stage = (stage + 1) % NORM_STAGES;
+#endif
+#if NORM_KEEP
+    norm_x kx[NORM_U], kd[NORM_U];
+#pragma unroll
+    for (int u = 0; u < NORM_U; ++u) {
+      const int j = u * STEP + g * NORM_VE;
+      if (there && j < n) {
+#if NORM_STAGES
+        memcpy(&kx[u], bx + u * ROW_THREADS, 16);
+        memcpy(&kd[u], bd + u * ROW_THREADS, 16);
+#else
+        kx[u] = norm_load(reinterpret_cast<const row_t*>(p.x) + row * p.n + j);
+        kd[u] = norm_load(reinterpret_cast<const row_t*>(p.dy) + row * p.n + j);
+#endif
+      }
+    }
+#if NORM_GAMMA_REGS
+#define NORM_GAMMA(u) for (int e = 0; e < NORM_VE; ++e) ga[e] = gr[u][e];
+#else
+#define NORM_GAMMA(u) norm_params(gamma + j, ga);     // (from L1: these lanes need their registers)
+#endif
+#define NORM_TAKE(u)     \
+  norm_wide(kx[u], v);   \
+  norm_wide(kd[u], d);   \
+  NORM_GAMMA(u)
+#else
+#define NORM_TAKE(u)                            \
+  row_unpack(bx[(u) * ROW_THREADS], v);         \
+  row_unpack(bd[(u) * ROW_THREADS], d);         \
+  norm_gamma(gs + j, ga);
+#endif
     f32 s[2] = {0.0f, 0.0f};
-    if (there) {
 #pragma unroll
-      for (int u = 0; u < NORM_U; ++u) {
-        const int j = u * STEP + g * NORM_VE;
-        if (j < n) {
-          f32 v[NORM_VE], d[NORM_VE], ga[NORM_VE];
-          norm_wide(bx[u], v);
-          norm_wide(bd[u], d);
-          norm_params(gamma + j, ga);
+    for (int u = 0; u < NORM_U; ++u) {
+      const int j = u * STEP + g * NORM_VE;
+      if (there && j < n) {
+        f32 v[NORM_VE], d[NORM_VE], ga[NORM_VE];
+        NORM_TAKE(u)
 #pragma unroll
-          for (int e = 0; e < NORM_VE; ++e) {
-            const f32 xh = (v[e] - mean) * rstd, a = d[e] * ga[e];
-            s[0] += a;
-            s[1] = fmaf(a, xh, s[1]);
-            sg[u * NORM_VE + e] = fmaf(d[e], xh, sg[u * NORM_VE + e]);
-            sb[u * NORM_VE + e] += d[e];
-          }
+        for (int e = 0; e < NORM_VE; ++e) {
+          const f32 xh = (v[e] - mean) * rstd, a = d[e] * ga[e];
+          s[0] += a;
+          s[1] = fmaf(a, xh, s[1]);
+          sg[u * NORM_VE + e] = fmaf(d[e], xh, sg[u * NORM_VE + e]);
+          sb[u * NORM_VE + e] += d[e];
         }
       }
     }
     norm_sum(s, red, slot);
     slot ^= 1;
     const f32 ma = s[0] / len, mb = s[1] / len;
-    if (there) {
-      row_t* dx = reinterpret_cast<row_t*>(p.dx) + row * p.n;
+    row_t* dx = reinterpret_cast<row_t*>(p.dx) + row * p.n;
 #pragma unroll
-      for (int u = 0; u < NORM_U; ++u) {
-        const int j = u * STEP + g * NORM_VE;
-        if (j < n) {
-          f32 v[NORM_VE], d[NORM_VE], ga[NORM_VE];
-          norm_wide(bx[u], v);
-          norm_wide(bd[u], d);
-          norm_params(gamma + j, ga);
+    for (int u = 0; u < NORM_U; ++u) {
+      const int j = u * STEP + g * NORM_VE;
+      if (there && j < n) {
+        f32 v[NORM_VE], d[NORM_VE], ga[NORM_VE];
+        NORM_TAKE(u)
 #pragma unroll
-          for (int e = 0; e < NORM_VE; ++e) v[e] = rstd * (fmaf(-((v[e] - mean) * rstd), mb, fmaf(d[e], ga[e], -ma)));
-          norm_store(dx + j, v);
-        }
+        for (int e = 0; e < NORM_VE; ++e) v[e] = rstd * (fmaf(-((v[e] - mean) * rstd), mb, fmaf(d[e], ga[e], -ma)));
+        norm_store(dx + j, v);
       }
     }
   }
   // this CTA's line: the groups' sums one after the other
   f32* line = reinterpret_cast<f32*>(p.partial) + (i64)blockIdx.x * 2 * p.n;
 #if NORM_ROWS > 1
-  extern __shared__ f32 sums[];          // 2 n Floats
+  f32* const sums = reinterpret_cast<f32*>(norm_memory);   // 2 n Floats, where the ring was
+#if NORM_STAGES
+  asm volatile("cp.async.wait_all;" ::: "memory");
+#endif
+  __syncthreads();
 #pragma unroll 1
   for (int q = 0; q < NORM_ROWS; ++q) {
     if (q == sub) {

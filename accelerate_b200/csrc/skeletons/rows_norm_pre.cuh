@@ -17,11 +17,12 @@ template <int N> struct norm_vec<u16, N> { typedef norm_bits16<N> type; };
 template <int N> struct norm_vec<f32, N> { typedef norm_bits32<N> type; };
 typedef norm_vec<row_t, NORM_VE>::type norm_x;
 
-// one access of x or dy: streamed, nobody reads it again
+// One access of x or dy: read once, so it takes no place in L1 (gamma and beta live there).
 __device__ __forceinline__ norm_x norm_load(const row_t* p) {
   norm_x r;
 #if NORM_VE > 1
-  const uint4 b = __ldcs(reinterpret_cast<const uint4*>(p));
+  uint4 b;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(b.x), "=r"(b.y), "=r"(b.z), "=r"(b.w) : "l"(p));
   memcpy(&r, &b, 16);
 #else
   r.v[0] = __ldcs(p);
@@ -58,6 +59,24 @@ __device__ __forceinline__ void norm_params(const param_t* p, f32 (&v)[NORM_VE])
     for (int e = 0; e < PER; ++e) v[h + e] = row_wide(b.v[e]);
   }
 }
+
+#if NORM_VE > 1
+// NORM_VE of them as Floats from shared memory
+__device__ __forceinline__ void norm_gamma(const f32* p, f32 (&v)[NORM_VE]) {
+#pragma unroll
+  for (int h = 0; h < NORM_VE; h += 4) {
+    const float4 q = *reinterpret_cast<const float4*>(p + h);
+    v[h] = q.x;
+    v[h + 1] = q.y;
+    v[h + 2] = q.z;
+    v[h + 3] = q.w;
+  }
+}
+// 16 bytes to shared memory without registers in between
+__device__ __forceinline__ void norm_copy(uint4* to, const row_t* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((u32)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+}
+#endif
 
 // Sums of a group's lanes, the same in every lane.  With several warps per row the warps' sums meet in shared memory;
 // `slot` alternates between calls, so that one barrier per call is enough.
