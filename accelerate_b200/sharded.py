@@ -84,8 +84,10 @@ class ProgramCache:
 class _View:
     """One leaf of a device array, described the way torch takes other libraries' device memory."""
 
-    def __init__(self, a, leaf):
-        self.__cuda_array_interface__ = {"shape": a.shape or (1,), "typestr": _TYPESTR[a.leaf_types[leaf]], "data": (a.devptr(leaf), False), "version": 3}
+    __slots__ = ("__cuda_array_interface__",)
+
+    def __init__(self, shape, typestr, ptr):
+        self.__cuda_array_interface__ = {"shape": shape, "typestr": typestr, "data": (ptr, False), "version": 3}
 
 
 _TYPESTR = {t: np.dtype(d).str for t, d in L.NP_OF.items()}
@@ -141,10 +143,11 @@ class GpuExecutor:
 
     def tensor(self, a, leaf=0):
         """Zero-copy torch view of one leaf of a device array."""
-        if 0 in a.shape:
+        shape = a.shape
+        if 0 in shape:
             dt = np.dtype(L.NP_OF[a.leaf_types[leaf]])
             return torch.empty(a.shape, dtype=torch.from_numpy(np.empty(0, dt)).dtype, device=self.stream.device)
-        t = torch.as_tensor(_View(a, leaf), device=self.device)
+        t = torch.as_tensor(_View(shape or (1,), _TYPESTR[a.leaf_types[leaf]], a.devptr(leaf)), device=self.device)
         t._keepalive = a
         return t
 
