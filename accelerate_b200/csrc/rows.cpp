@@ -295,6 +295,9 @@ void Program::exec_foreign(const Node& n, Env& env) {
   for (auto& name : n.args) a.push_back(env.at(name));
   const DevArray& x = *a[n.foreign == F_LOG_PROBS || n.foreign == F_LAYER_NORM_GRAD ? 1 : 2];
   const std::vector<int64_t> outer(x.shape.begin(), x.shape.end() - 1);
+  for (auto& b : a)
+    for (size_t l = 0; l < b->leaf.size(); ++l)
+      if ((uintptr_t)b->leaf[l]->ptr % ty_bytes[b->leaf_ty[l]]) throw Error(B200_ERR_ARG, "an array does not start on a boundary of its elements");
   const int64_t cols = std::max<int64_t>(x.shape.back(), 0);
   int64_t rows = 1;
   for (int64_t d : outer) rows *= std::max<int64_t>(d, 0);

@@ -34,7 +34,7 @@ extern "C" __global__ void __launch_bounds__(ROW_THREADS, ROW_MIN_BLOCKS) acc_ro
     if (i < b1) nxt[u] = span.load(i);
   }
   const f32 lse = reinterpret_cast<const f32*>(p.lse)[row];
-  const f32 scale = reinterpret_cast<const f32*>(p.g)[row] * tau;
+  f32 scale = reinterpret_cast<const f32*>(p.g)[row] * tau;
   // the teacher's distribution: maximum and sum over the entries that are there
   f32 mt = -ROW_INF;
   bool bad = false;
@@ -63,6 +63,7 @@ extern "C" __global__ void __launch_bounds__(ROW_THREADS, ROW_MIN_BLOCKS) acc_ro
 #pragma unroll
   for (int w = 0; w < DG_WARPS; ++w) es += red[1][w];
   const bool has = es != 0.0f;
+  if (es != es) scale = es;              // a NaN among the teacher's logits: no gradient is a number
   if (bad && tid == 0 && part == 0) acc_fail(p.err, 1003);
 
   // p_j g tau = 2^(c (s - tau lse)) g tau: the product tau lse is not rounded before the subtraction, so the exponent

@@ -13,6 +13,7 @@ is one row, a matrix ``Z :. rows :. n`` many.  All arguments of a call have the 
 from __future__ import annotations
 
 import math
+import numbers
 
 from .language import (INT, Exp, _control, _avars, compute, cond, constant, exp, fold, from_index, from_integral, generate, index, is_nan, lift,
                        log, lor, land, lnot, max_, map_, shape_size, sqrt, tup, use, _as_list)
@@ -101,9 +102,11 @@ def logProbs(k, tokens, logits):
     with nothing else has lse and log probabilities of -inf and entropy 0.  NaN and +inf make a row's numbers NaN;
     among the alternatives a NaN comes first.  A row shorter than k ends in alternatives (-1, -inf)."""
     tokens, logits = use(tokens), use(logits)
-    _need(isinstance(k, int) and 0 <= k <= 128, "logProbs: the number of alternatives is a whole number from 0 to 128")
+    _need(isinstance(k, numbers.Integral) and 0 <= k <= 128, "logProbs: the number of alternatives is a whole number from 0 to 128")
     _need(logits.rank >= 1 and logits.elt in _REAL, "logProbs: the logits must be an array of Half or Float of rank 1 or more")
     _need(tokens.rank == logits.rank - 1 and tokens.elt in ("i32", "i64"), "logProbs: the given tokens must be Int32 or Int, one per row")
+
+    k = int(k)
 
     def definition(tok, xs):
         r = xs.rank
@@ -152,7 +155,7 @@ def _teacher(tau, ids, ts):
 
 
 def _check_distill(what, tau, ids, teacher, student):
-    _need(isinstance(tau, (int, float)) and 1e-4 <= tau <= 1e4, f"{what}: the temperature must lie between 1e-4 and 1e4")
+    _need(isinstance(tau, numbers.Real) and 1e-4 <= tau <= 1e4, f"{what}: the temperature must lie between 1e-4 and 1e4")
     _need(student.rank >= 1 and student.elt in _REAL, f"{what}: the student's logits must be an array of Half or Float of rank 1 or more")
     _need(ids.rank == student.rank and ids.elt == "i32", f"{what}: the teacher's tokens must be Int32, one list per row")
     _need(teacher.rank == student.rank and teacher.elt in _REAL, f"{what}: the teacher's logits must be Half or Float, one list per row")
@@ -229,7 +232,7 @@ def layerNorm(eps, gamma, beta, xs):
     gamma and beta have the rows' length and either the rows' type or Float.  The result is rounded once to the rows' type.
     eps may be 0 (a constant row is then NaN).  Rows of length zero have NaN statistics."""
     gamma, beta, xs = use(gamma), use(beta), use(xs)
-    _need(isinstance(eps, (int, float)) and 0 <= eps <= 3.4e38, "layerNorm: epsilon must be finite and not negative")
+    _need(isinstance(eps, numbers.Real) and 0 <= eps <= 3.4e38, "layerNorm: epsilon must be finite and not negative")
     _need(xs.rank >= 1 and xs.elt in _REAL, "layerNorm: the rows must be an array of Half or Float of rank 1 or more")
     _need(gamma.rank == 1 and gamma.elt in (xs.elt, "f32") and beta.rank == 1 and beta.elt == gamma.elt,
           "layerNorm: gamma and beta must be vectors of the rows' type or of Float")

@@ -300,6 +300,48 @@ def test_a_capture_is_refused(gpu_ctx):
     assert np.array_equal(y.download(), np.ones((2, 8), np.float32))
 
 
+def test_memory_that_cannot_be_an_array_is_refused(gpu_ctx):
+    import torch
+
+    from accelerate_b200 import sharded
+    ex = sharded.GpuExecutor(gpu_ctx)
+    t = torch.zeros(4, 6, device="cuda")
+    torch.cuda.synchronize()
+    with pytest.raises(ValueError):
+        ex.wrap(t.t(), "f32")
+    with pytest.raises(ValueError):
+        gpu_ctx.wrap(("f32", "f32"), (4,), [t.data_ptr()])
+    prog = A.build_program(list(A.layerNorm(1e-5, A.param(1, "f32"), A.param(1, "f32"), A.param(2, "f32"))))
+    v = gpu_ctx.from_host(np.ones(5, np.float32))
+    off = gpu_ctx.wrap("f32", (2, 5), [t.data_ptr() + 2])
+    with pytest.raises(backend.B200Error) as e:
+        gpu_ctx.execute(prog.text, [v, v, off], 2)
+    assert e.value.code == 7 and "boundary" in str(e.value)
+
+
+def test_inside_a_loop(gpu_ctx):
+    """Foreign functions in the body of an awhile: the state goes through the kernel every trip."""
+    g = G(22)
+    x, ga, be = g.normal(size=(3, 40)).astype(np.float32), np.full(40, 1.5, np.float32), np.full(40, 0.25, np.float32)
+
+    def loop():
+        return A.awhile(lambda s: A.unit(A.the(s[1]) < 3), lambda s: (A.layerNorm(1e-5, ga, be, s[0])[0], A.map(lambda n: n + 1, s[1])),
+                        (A.use(x), A.unit(A.constant(0))))
+    got, want = backend.run(list(loop())), oracle.run(list(loop()))
+    # three norms, each a sum of 40 Floats of size at most 10, applied to the last one's error
+    assert int(got[1]) == 3 and np.max(np.abs(got[0].astype(np.float64) - want[0])) < 3 * 60 * 2.0 ** -24 * 10
+
+
+def test_a_teacher_that_is_not_a_number(gpu_ctx):
+    x = np.zeros((3, 70), np.float32)
+    ids, te = np.array([[1, 2], [3, 3], [-1, 5]], np.int32), np.array([[np.nan, 0], [np.inf, 1], [np.nan, 0]], np.float32)
+    loss, lse = RUN(A.distill(1.0, ids, te, x))
+    assert np.isnan(loss).tolist() == [True, True, False]
+    d = RUN([A.distillGrad(1.0, ids, te, x, lse, np.ones(3, np.float32))])[0]
+    want = oracle.run(A.distillGrad(1.0, ids, te, x, lse, np.ones(3, np.float32)))
+    assert np.all(np.isnan(d[:2])) and np.all(np.isnan(want[:2])) and np.allclose(d[2], want[2], atol=1e-6)
+
+
 def test_calls_from_two_threads_and_two_contexts(gpu_ctx):
     import threading
     g = G(20)

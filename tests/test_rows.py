@@ -139,6 +139,12 @@ def test_arguments_are_checked():
             f()
 
 
+def test_numpy_numbers_are_numbers():
+    x = np.zeros((2, 4), np.float32)
+    A.logProbs(np.int64(2), np.zeros(2, np.int32), x)
+    A.distill(np.float32(2), np.zeros((2, 1), np.int32), np.zeros((2, 1), np.float32), x)
+
+
 def _texts():
     out = {}
     for t in ("f16", "f32"):
