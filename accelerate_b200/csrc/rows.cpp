@@ -191,38 +191,47 @@ NormShape norm_shape(int64_t n, int ve, int most_elems, int most_warps, int64_t 
   return s;
 }
 constexpr int kNormElems = 32, kNormWarps = 32;          // forward: elements per thread, warps per row
+// Elements per access: the widest, up to 16 bytes, on whose boundary all rows and the parameters start.
+int norm_access(const std::vector<const DevArray*>& rows_like, const std::vector<const DevArray*>& params, int64_t cols, int elt_bytes, int param_bytes) {
+  uint64_t at = (uint64_t)cols * elt_bytes, pat = 0;
+  for (auto* a : rows_like) at |= (uint64_t)(uintptr_t)a->leaf[0]->ptr;
+  for (auto* a : params) pat |= (uint64_t)(uintptr_t)a->leaf[0]->ptr;
+  int ve = 16 / elt_bytes;
+  while (ve > 1 && (at % (ve * elt_bytes) != 0 || pat % std::min(16, ve * param_bytes) != 0)) ve /= 2;
+  return ve;
+}
 NormShape norm_forward_shape(int64_t n, int ve, int64_t rows, int sms) {
-  const NormShape s = norm_shape(n, ve, ve == 1 ? 8 : 32, 8, rows, sms);
+  const NormShape s = norm_shape(n, ve, ve <= 2 ? 8 * ve : 32, 8, rows, sms);
   return s.whole ? s : norm_shape(n, ve, kNormElems, kNormWarps, rows, sms);
 }
 constexpr int kNormGradElems = 16, kNormGradWarps = 16;  // gradients; twice the elements where they pass through shared memory
 // Shared memory per CTA for rows in flight: two CTAs of 256 threads per SM, or one of 512
 constexpr int64_t kRingBytes = 104 << 10, kRingBytesAlone = 208 << 10;
-NormShape norm_grad_shape(int64_t n, int ve, int64_t rows, int sms) {
-  if (ve == 1) {
-    // (one element per access: eight per lane leave the registers for three CTAs per SM)
-    const NormShape s = norm_shape(n, ve, kNormGradElems / 2, kNormGradWarps, rows, sms);
-    return s.whole ? s : norm_shape(n, ve, kNormGradElems, kNormGradWarps, rows, sms);
-  }
+NormShape norm_grad_shape(int64_t n, int ve, int elt_bytes, int64_t rows, int sms) {
+  const int bytes = ve * elt_bytes;
   NormShape s = norm_shape(n, ve, kNormGradElems, kNormGradWarps, rows, sms);
+  if (bytes == 2) {
+    // (Halves one by one: eight per lane leave the registers for two CTAs per SM)
+    const NormShape few = norm_shape(n, ve, kNormGradElems / 2, kNormGradWarps, rows, sms);
+    return few.whole ? few : s;
+  }
   int64_t rest = 0;
   if (!s.whole) {
+    const NormShape reread = s;
+    if (bytes < 16) return reread;
     s = norm_shape(n, ve, 2 * kNormGradElems, kNormGradWarps, rows, sms);
     if (!s.whole) return s;
     s.keep = false;
     rest = 4LL * s.u * s.threads * ve;       // gamma, for any length that comes to this shape
+    if (kRingBytesAlone - rest < 2 * 2LL * bytes * s.u * s.threads) return reread;
   }
-  const int64_t stage = 2LL * 16 * s.u * s.threads, room = (s.threads > kThreads ? kRingBytesAlone : kRingBytes) - rest;
+  const int64_t stage = 2LL * bytes * s.u * s.threads, room = (s.threads > kThreads ? kRingBytesAlone : kRingBytes) - rest;
   s.stages = (int)std::min<int64_t>(4, room / stage);
-  if (s.stages < 2) {
-    NormShape reread = {ve, 16, 1, 512, false};
-    return reread;
-  }
   return s;
 }
-size_t norm_grad_smem(const NormShape& s, int64_t n) {
+size_t norm_grad_smem(const NormShape& s, int elt_bytes, int64_t n) {
   if (!s.whole) return 0;
-  const size_t ring = 2u * 16 * s.u * s.threads * s.stages + (s.keep ? 0 : 4u * s.u * s.threads * s.ve), sums = s.rows() > 1 ? (size_t)n * 8 : 0;
+  const size_t ring = 2u * s.ve * elt_bytes * s.u * s.threads * s.stages + (s.keep ? 0 : 4u * s.u * s.threads * s.ve), sums = s.rows() > 1 ? (size_t)n * 8 : 0;
   return std::max(ring, sums);
 }
 
@@ -239,11 +248,11 @@ std::vector<std::pair<std::string, Variant>> foreign_variants(const Node& n) {
     case F_DISTILL_GRAD: v.push_back({"rows_distill_grad", distill_grad_variant(1)}); break;
     case F_LAYER_NORM:
       for (int64_t len : {1024, 4096, 1 << 20})
-        for (int w : {ve, 1}) v.push_back({"rows_norm", norm_forward_shape(len, w, 1 << 20, 148).variant()});
+        for (int w : {ve, 2, 1}) v.push_back({"rows_norm", norm_forward_shape(len, w, 1 << 20, 148).variant()});
       break;
     case F_LAYER_NORM_GRAD:
       for (int64_t len : {1024, 4096, 12000, 1 << 20})
-        for (int w : {ve, 1}) v.push_back({"rows_norm_grad", with(norm_grad_shape(len, w, 1 << 20, 148).variant(), "")});
+        for (int w : {ve, 2, 1}) v.push_back({"rows_norm_grad", with(norm_grad_shape(len, w, 16 / ve, 1 << 20, 148).variant(), "")});
       v.push_back({"rows_norm_grad", with(NormShape{1, 1, 1, 1024, true}.variant(), "NORM_SUMS")});
       v.push_back({"rows_norm_grad", with(NormShape{1, 1, 1, kThreads, true}.variant(), "NORM_COLS")});
       break;
@@ -362,8 +371,8 @@ void Program::exec_foreign(const Node& n, Env& env) {
       env[n.outs[0]] = y;
       env[n.outs[1]] = stats;
       if (rows == 0) break;
-      const bool wide = x.aligned16() && y->aligned16() && a[0]->aligned16() && a[1]->aligned16() && cols * elt_bytes % 16 == 0;
-      const NormShape s = norm_forward_shape(cols, wide ? 16 / elt_bytes : 1, rows, c.sm_count);
+      const int ve = norm_access({&x, y.get()}, {a[0].get(), a[1].get()}, cols, elt_bytes, ty_bytes[a[0]->elt.s]);
+      const NormShape s = norm_forward_shape(cols, ve, rows, c.sm_count);
       CompiledKernel& ker = shape_kernel(c, st, s.key(), "rows_norm", [&] { return s.variant(); }, "acc_rows_norm", s.threads, 0);
       launch(c, ker, (rows + s.rows() - 1) / s.rows(), s.threads, 0,
              {ptr_of(x), ptr_of(*a[0]), ptr_of(*a[1]), ptr_of(*y), ptr_of(*stats, 0), ptr_of(*stats, 1), (uint64_t)rows, (uint64_t)cols, float_bits(n.consts[0])});
@@ -378,8 +387,8 @@ void Program::exec_foreign(const Node& n, Env& env) {
       env[n.outs[1]] = dgamma;
       env[n.outs[2]] = dbeta;
       if (cols == 0) break;
-      const bool wide = x.aligned16() && dx->aligned16() && a[3]->aligned16() && a[0]->aligned16() && cols * elt_bytes % 16 == 0;
-      const NormShape s = norm_grad_shape(cols, wide ? 16 / elt_bytes : 1, rows, c.sm_count);
+      const int ve = norm_access({&x, dx.get(), a[3].get()}, {a[0].get()}, cols, elt_bytes, ty_bytes[a[0]->elt.s]);
+      const NormShape s = norm_grad_shape(cols, ve, elt_bytes, rows, c.sm_count);
       // (one source for three kernels: which of them it compiles to)
       auto which = [&](bool sums, bool cols_) {
         return [&, sums, cols_] {
@@ -389,7 +398,7 @@ void Program::exec_foreign(const Node& n, Env& env) {
           return v;
         };
       };
-      const size_t smem = norm_grad_smem(s, cols);
+      const size_t smem = norm_grad_smem(s, elt_bytes, cols);
       CompiledKernel& ker = shape_kernel(c, st, s.key(), "rows_norm_grad", which(false, false), "acc_rows_norm_grad", s.threads, smem);
       // as many CTAs as fit at once, and few enough for four trips each: a CTA costs a line of partial sums
       const int64_t groups = (rows + s.rows() - 1) / s.rows();

@@ -5,9 +5,9 @@
 // `partial` (one line of 2 n Floats per CTA) and acc_rows_norm_sums adds the lines in their order: the same
 // numbers every time, whatever order the CTAs ran in.
 //
-//   NORM_STAGES  rows of x and dy on their way while one is worked on: every lane copies its own 16-byte blocks to
-//                shared memory (cp.async) and reads them back itself, so the ring needs no barrier and no flag.  0: rows
-//                that do not start on 16-byte boundaries are loaded directly.
+//   NORM_STAGES  rows of x and dy on their way while one is worked on: every lane copies its own elements to shared
+//                memory (cp.async) and reads them back itself, so the ring needs no barrier and no flag.  0: rows of
+//                Halves that start on odd elements (no such copy of 2 bytes exists) are loaded directly.
 //   NORM_KEEP    1: a row's blocks and gamma stay in registers between the two passes (up to 16 elements per lane);
 //                0: gamma lies in shared memory and the blocks are read from the ring twice (32 elements per lane,
 //                whose sums alone take 64 registers)
@@ -126,7 +126,7 @@ extern "C" __global__ void __launch_bounds__(ROW_THREADS, ROW_THREADS > 256 ? 1 
   const i64 stride = (i64)gridDim.x * NORM_ROWS;
 #if NORM_STAGES
   // the ring: [stage][x, dy][access][thread], behind it gamma
-  uint4* const mine = norm_memory + threadIdx.x;
+  norm_x* const mine = reinterpret_cast<norm_x*>(norm_memory) + threadIdx.x;
   constexpr int PLANE = NORM_U * ROW_THREADS;
   auto fetch = [&](i64 r, int stage) {
     if (r < p.rows) {
@@ -148,7 +148,7 @@ extern "C" __global__ void __launch_bounds__(ROW_THREADS, ROW_THREADS > 256 ? 1 
   int stage = 0;
 #endif
 #if !NORM_KEEP
-  f32* const gs = reinterpret_cast<f32*>(norm_memory + 2 * NORM_STAGES * PLANE);
+  f32* const gs = reinterpret_cast<f32*>(reinterpret_cast<norm_x*>(norm_memory) + 2 * NORM_STAGES * PLANE);
   for (int j = threadIdx.x; j < n; j += ROW_THREADS) gs[j] = row_wide(gamma[j]);
   __syncthreads();
 #elif NORM_GAMMA_REGS
@@ -178,8 +178,8 @@ extern "C" __global__ void __launch_bounds__(ROW_THREADS, ROW_THREADS > 256 ? 1 
     // (the stage fetched into now was read in the trip before, by this thread)
     fetch(row + (NORM_STAGES - 1) * stride, (stage + NORM_STAGES - 1) % NORM_STAGES);
     asm volatile("cp.async.wait_group %0;" ::"n"(NORM_STAGES - 1) : "memory");
-    const uint4* const bx = mine + (2 * stage) * PLANE;
-    const uint4* const bd = mine + (2 * stage + 1) * PLANE;
+    const norm_x* const bx = mine + (2 * stage) * PLANE;
+    const norm_x* const bd = mine + (2 * stage + 1) * PLANE;
     stage = (stage + 1) % NORM_STAGES;
 #endif
 #if NORM_KEEP
@@ -189,8 +189,8 @@ extern "C" __global__ void __launch_bounds__(ROW_THREADS, ROW_THREADS > 256 ? 1 
       const int j = u * STEP + g * NORM_VE;
       if (there && j < n) {
 #if NORM_STAGES
-        memcpy(&kx[u], bx + u * ROW_THREADS, 16);
-        memcpy(&kd[u], bd + u * ROW_THREADS, 16);
+        kx[u] = bx[u * ROW_THREADS];
+        kd[u] = bd[u * ROW_THREADS];
 #else
         kx[u] = norm_load(reinterpret_cast<const row_t*>(p.x) + row * p.n + j);
         kd[u] = norm_load(reinterpret_cast<const row_t*>(p.dy) + row * p.n + j);
@@ -208,8 +208,8 @@ extern "C" __global__ void __launch_bounds__(ROW_THREADS, ROW_THREADS > 256 ? 1 
   NORM_GAMMA(u)
 #else
 #define NORM_TAKE(u)                            \
-  row_unpack(bx[(u) * ROW_THREADS], v);         \
-  row_unpack(bd[(u) * ROW_THREADS], d);         \
+  norm_wide(bx[(u) * ROW_THREADS], v);          \
+  norm_wide(bd[(u) * ROW_THREADS], d);          \
   norm_gamma(gs + j, ga);
 #endif
     f32 s[2] = {0.0f, 0.0f};

@@ -1,9 +1,9 @@
 // What the layer norm kernels share: a row spread over NORM_WARPS warps (NORM_GROUP lanes), NORM_U accesses of
 // NORM_VE elements per lane.  Lane g holds the elements [(u * NORM_GROUP + g) * NORM_VE, + NORM_VE).
 //
-//   NORM_VE     elements per access: 16 bytes' worth if every row and both parameter vectors start on 16-byte
-//               boundaries, else 1; neighbouring lanes then hold neighbouring elements, so the narrow accesses of a
-//               warp still cover whole sectors
+//   NORM_VE     elements per access, a power of two: the widest access, up to 16 bytes, on whose boundary every row
+//               and both parameter vectors start; neighbouring lanes hold neighbouring accesses, so that narrow ones
+//               still cover whole sectors
 //   NORM_WARPS  warps per row, a power of two; NORM_ROWS rows per CTA at a time
 //   NORM_U      accesses per lane;  NORM_GROUP * NORM_U * NORM_VE >= n
 
@@ -15,38 +15,64 @@ template <int N> struct __align__(4 * N) norm_bits32 { f32 v[N]; };
 template <class T, int N> struct norm_vec;
 template <int N> struct norm_vec<u16, N> { typedef norm_bits16<N> type; };
 template <int N> struct norm_vec<f32, N> { typedef norm_bits32<N> type; };
-typedef norm_vec<row_t, NORM_VE>::type norm_x;
+#if ROW_F16
+#define NORM_BYTES (2 * NORM_VE)
+#else
+#define NORM_BYTES (4 * NORM_VE)
+#endif
+#if NORM_BYTES == 16
+typedef uint4 norm_x;
+#elif NORM_BYTES == 8
+typedef uint2 norm_x;
+#elif NORM_BYTES == 4
+typedef u32 norm_x;
+#else
+typedef u16 norm_x;
+#endif
 
 // One access of x or dy: read once, so it takes no place in L1 (gamma and beta live there).
 __device__ __forceinline__ norm_x norm_load(const row_t* p) {
-  norm_x r;
-#if NORM_VE > 1
+#if NORM_BYTES == 16
   uint4 b;
   asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(b.x), "=r"(b.y), "=r"(b.z), "=r"(b.w) : "l"(p));
-  memcpy(&r, &b, 16);
+  return b;
 #else
-  r.v[0] = __ldcs(p);
+  return __ldcs(reinterpret_cast<const norm_x*>(p));
 #endif
-  return r;
 }
 __device__ __forceinline__ void norm_wide(const norm_x& b, f32 (&v)[NORM_VE]) {
-#if ROW_F16 && NORM_VE > 1
-  uint4 w;
-  memcpy(&w, &b, 16);
-  row_unpack(w, v);
+#if NORM_BYTES == 2
+  v[0] = row_h2f(b);
 #else
+  u32 w[NORM_BYTES / 4];
+  memcpy(w, &b, NORM_BYTES);
 #pragma unroll
-  for (int e = 0; e < NORM_VE; ++e) v[e] = row_wide(b.v[e]);
+  for (int i = 0; i < NORM_BYTES / 4; ++i) {
+#if ROW_F16
+    row_h2x2(w[i], v[2 * i], v[2 * i + 1]);
+#else
+    v[i] = __uint_as_float(w[i]);
+#endif
+  }
 #endif
 }
 __device__ __forceinline__ void norm_store(row_t* p, const f32 (&v)[NORM_VE]) {
-#if NORM_VE > 1
-  __stcs(reinterpret_cast<uint4*>(p), row_pack(v));
+  norm_x b;
+#if NORM_BYTES == 2
+  b = row_f2h(v[0]);
 #else
-  row_t o;
-  row_narrow(v[0], o);
-  __stcs(p, o);
+  u32 w[NORM_BYTES / 4];
+#pragma unroll
+  for (int i = 0; i < NORM_BYTES / 4; ++i) {
+#if ROW_F16
+    w[i] = row_x2h2(v[2 * i], v[2 * i + 1]);
+#else
+    w[i] = __float_as_uint(v[i]);
 #endif
+  }
+  memcpy(&b, w, NORM_BYTES);
+#endif
+  __stcs(reinterpret_cast<norm_x*>(p), b);
 }
 // NORM_VE parameters (gamma, beta) from j on
 __device__ __forceinline__ void norm_params(const param_t* p, f32 (&v)[NORM_VE]) {
@@ -60,21 +86,30 @@ __device__ __forceinline__ void norm_params(const param_t* p, f32 (&v)[NORM_VE])
   }
 }
 
-#if NORM_VE > 1
 // NORM_VE of them as Floats from shared memory
 __device__ __forceinline__ void norm_gamma(const f32* p, f32 (&v)[NORM_VE]) {
 #pragma unroll
-  for (int h = 0; h < NORM_VE; h += 4) {
-    const float4 q = *reinterpret_cast<const float4*>(p + h);
-    v[h] = q.x;
-    v[h + 1] = q.y;
-    v[h + 2] = q.z;
-    v[h + 3] = q.w;
+  for (int e = 0; e < NORM_VE; e += 4) {
+    if (NORM_VE >= 4) {
+      const float4 q = *reinterpret_cast<const float4*>(p + e);
+      v[e] = q.x;
+      v[(e + 1) % NORM_VE] = q.y;
+      v[(e + 2) % NORM_VE] = q.z;
+      v[(e + 3) % NORM_VE] = q.w;
+    } else {
+      for (int i = 0; i < NORM_VE; ++i) v[i] = p[i];
+    }
   }
 }
-// 16 bytes to shared memory without registers in between
-__device__ __forceinline__ void norm_copy(uint4* to, const row_t* from) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((u32)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+#if NORM_BYTES >= 4
+// One access to shared memory without registers in between
+__device__ __forceinline__ void norm_copy(norm_x* to, const row_t* from) {
+  const u32 at = (u32)__cvta_generic_to_shared(to);
+#if NORM_BYTES == 16
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at), "l"(from) : "memory");
+#else
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(at), "l"(from), "n"(NORM_BYTES) : "memory");
+#endif
 }
 #endif
 

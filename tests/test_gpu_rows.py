@@ -152,7 +152,7 @@ def test_distill_of_masked_and_large_rows(gpu_ctx, t):
 
 
 @pytest.mark.parametrize("t,pt", [("f16", "f16"), ("f16", "f32"), ("f32", "f32")])
-@pytest.mark.parametrize("rows,n", [(1, 1), (3, 5), (2, 8), (1000, 33), (37, 768), (5, 1000), (300, 1001), (9, 4096), (700, 2048), (3, 8192), (2, 8200), (2, 16384), (2, 20001), (1, 40000), (3, 140000)])
+@pytest.mark.parametrize("rows,n", [(1, 1), (3, 5), (2, 8), (1000, 33), (37, 768), (5, 1000), (300, 1001), (300, 1002), (300, 1004), (9, 4096), (700, 2048), (3, 8192), (2, 8194), (2, 8200), (2, 12296), (2, 16384), (2, 20001), (1, 40000), (3, 140000)])
 def test_layer_norm_and_its_gradient(gpu_ctx, t, pt, rows, n):
     g = G(rows + n)
     x = (g.normal(size=(rows, n)) * g.uniform(0.5, 2, (rows, 1)) + 0.4).astype(R.NP[t])
@@ -283,6 +283,7 @@ def test_shapes_that_do_not_match_are_refused(gpu_ctx):
         assert e.value.code == 5 and "shape mismatch" in str(e.value)
 
 
+@pytest.mark.filterwarnings("ignore:The CUDA Graph is empty")
 def test_a_capture_is_refused(gpu_ctx):
     import torch
     stream = torch.cuda.ExternalStream(gpu_ctx.stream())
