@@ -141,13 +141,14 @@ constexpr int kThreads = 256, kStatsThreads = 128;
 Variant stats_variant(int ctas) { return {{"ROW_THREADS", str(kStatsThreads)}, {"ROW_U", "8"}, {"ROW_MIN_BLOCKS", "7"}, {"ROW_C", str(ctas)}}; }
 Variant distill_grad_variant(int ctas) { return {{"ROW_THREADS", str(kThreads)}, {"ROW_U", "4"}, {"ROW_MIN_BLOCKS", "4"}, {"ROW_C", str(ctas)}}; }
 
-// CTAs that share a row: enough to give every SM `several`, as long as each has a tile of its own.  The statistics
-// take 4 (500 rows of 50257 Floats, k = 5: 2 CTAs per row 28.7 us, 4 CTAs 42 us: every CTA finds a threshold of its
-// own), the gradient 8 (333 rows of 50257: 31.6 us with 8, 35.0 with 4).
-int ctas_per_row(int64_t rows, int64_t n, int elt_bytes, int sms, int several, int most) {
+// CTAs that share a row: at least `least`, and enough to give every SM `several`, as long as each has a tile of its own.
+// The statistics take as few as fill the machine (500 rows of 50257 Floats, k = 5: 2 CTAs per row 28.7 us, 4 CTAs
+// 42 us: every CTA finds a threshold of its own); the gradient, whose CTAs are independent, four (4096 rows of
+// 131072 Halves: 372 us with one CTA per row, 357 with four, 524 with sixteen).
+int ctas_per_row(int64_t rows, int64_t n, int elt_bytes, int sms, int least, int several, int most) {
   const int64_t tiles = (n * elt_bytes + 16 * kThreads * 4 - 1) / (16 * kThreads * 4);
   int c = 1;
-  while (c < most && rows * c < several * (int64_t)sms && 2 * c <= tiles) c *= 2;
+  while (c < most && (c < least || rows * c < several * (int64_t)sms) && 2 * c <= tiles) c *= 2;
   return c;
 }
 
@@ -209,12 +210,10 @@ constexpr int kNormGradElems = 16, kNormGradWarps = 16;  // gradients; twice the
 constexpr int64_t kRingBytes = 104 << 10, kRingBytesAlone = 208 << 10;
 NormShape norm_grad_shape(int64_t n, int ve, int elt_bytes, int64_t rows, int sms) {
   const int bytes = ve * elt_bytes;
-  NormShape s = norm_shape(n, ve, kNormGradElems, kNormGradWarps, rows, sms);
-  if (bytes == 2) {
-    // (Halves one by one: eight per lane leave the registers for two CTAs per SM)
-    const NormShape few = norm_shape(n, ve, kNormGradElems / 2, kNormGradWarps, rows, sms);
-    return few.whole ? few : s;
-  }
+  // (accesses of one element: eight per lane, which leave registers for more rows at a time, as long as the row fits)
+  NormShape s = norm_shape(n, ve, std::min(kNormGradElems, 8 * ve), kNormGradWarps, rows, sms);
+  if (!s.whole) s = norm_shape(n, ve, kNormGradElems, kNormGradWarps, rows, sms);
+  if (bytes == 2) return s;
   int64_t rest = 0;
   if (!s.whole) {
     const NormShape reread = s;
@@ -326,7 +325,7 @@ void Program::exec_foreign(const Node& n, Env& env) {
       env[n.outs[0]] = stats;
       env[n.outs[1]] = top;
       if (rows == 0) break;
-      const int ctas = ctas_per_row(rows, cols, elt_bytes, c.sm_count, 4, 8);
+      const int ctas = ctas_per_row(rows, cols, elt_bytes, c.sm_count, 1, 4, 8);
       const size_t smem = stats_smem(k > 0);
       CompiledKernel& ker = shape_kernel(c, st, (uint64_t)ctas, "rows_stats", [&] { return stats_variant(ctas); }, "acc_rows_stats", kStatsThreads, smem);
       launch(c, ker, rows * ctas, kStatsThreads, smem,
@@ -345,7 +344,7 @@ void Program::exec_foreign(const Node& n, Env& env) {
         env[n.outs[0]] = loss;
         env[n.outs[1]] = lse;
         if (rows == 0) break;
-        const int ctas = ctas_per_row(rows, cols, elt_bytes, c.sm_count, 4, 8);
+        const int ctas = ctas_per_row(rows, cols, elt_bytes, c.sm_count, 1, 4, 8);
         const size_t smem = stats_smem(false);
         CompiledKernel& ker = shape_kernel(c, st, (uint64_t)ctas, "rows_stats", [&] { return stats_variant(ctas); }, "acc_rows_stats", kStatsThreads, smem);
         launch(c, ker, rows * ctas, kStatsThreads, smem,
@@ -357,7 +356,7 @@ void Program::exec_foreign(const Node& n, Env& env) {
         DevArrayP dx = c.new_array(n.out_info[0].elt, x.shape);
         env[n.outs[0]] = dx;
         if (rows == 0 || cols == 0) break;
-        const int ctas = ctas_per_row(rows, cols, elt_bytes, c.sm_count, 8, 16);
+        const int ctas = ctas_per_row(rows, cols, elt_bytes, c.sm_count, 4, 8, 16);
         CompiledKernel& ker = shape_kernel(c, st, (uint64_t)ctas, "rows_distill_grad", [&] { return distill_grad_variant(ctas); }, "acc_rows_distill_grad", kThreads, 0);
         launch(c, ker, rows * ctas, kThreads, 0,
                {ptr_of(x), ptr_of(*a[0]), ptr_of(*a[1]), ptr_of(*a[3]), ptr_of(*a[4]), ptr_of(*dx), (uint64_t)rows, (uint64_t)cols, (uint64_t)k,

@@ -189,8 +189,8 @@ extern "C" __global__ void __launch_bounds__(ROW_THREADS, ROW_THREADS > 256 ? 1 
       const int j = u * STEP + g * NORM_VE;
       if (there && j < n) {
 #if NORM_STAGES
-        kx[u] = bx[u * ROW_THREADS];
-        kd[u] = bd[u * ROW_THREADS];
+        kx[u] = norm_shared(bx + u * ROW_THREADS);
+        kd[u] = norm_shared(bd + u * ROW_THREADS);
 #else
         kx[u] = norm_load(reinterpret_cast<const row_t*>(p.x) + row * p.n + j);
         kd[u] = norm_load(reinterpret_cast<const row_t*>(p.dy) + row * p.n + j);
@@ -207,9 +207,9 @@ extern "C" __global__ void __launch_bounds__(ROW_THREADS, ROW_THREADS > 256 ? 1 
   norm_wide(kd[u], d);   \
   NORM_GAMMA(u)
 #else
-#define NORM_TAKE(u)                            \
-  norm_wide(bx[(u) * ROW_THREADS], v);          \
-  norm_wide(bd[(u) * ROW_THREADS], d);          \
+#define NORM_TAKE(u)                                 \
+  norm_wide(norm_shared(bx + (u) * ROW_THREADS), v); \
+  norm_wide(norm_shared(bd + (u) * ROW_THREADS), d); \
   norm_gamma(gs + j, ga);
 #endif
     f32 s[2] = {0.0f, 0.0f};

@@ -20,59 +20,67 @@ template <int N> struct norm_vec<f32, N> { typedef norm_bits32<N> type; };
 #else
 #define NORM_BYTES (4 * NORM_VE)
 #endif
-#if NORM_BYTES == 16
-typedef uint4 norm_x;
-#elif NORM_BYTES == 8
-typedef uint2 norm_x;
-#elif NORM_BYTES == 4
-typedef u32 norm_x;
+template <int B> struct norm_raw;
+template <> struct norm_raw<16> { typedef uint4 type; };
+template <> struct norm_raw<8> { typedef uint2 type; };
+template <> struct norm_raw<4> { typedef u32 type; };
+template <> struct norm_raw<2> { typedef u16 type; };
+typedef norm_raw<NORM_BYTES>::type norm_word;
+// What came with one access.  Halves stay in the words they came in; Floats are kept as Floats (as words, the
+// compiler's schedule cost the forward kernel 6 to 10 %).
+#if ROW_F16
+typedef norm_word norm_x;
 #else
-typedef u16 norm_x;
+typedef norm_vec<f32, NORM_VE>::type norm_x;
 #endif
 
 // One access of x or dy: read once, so it takes no place in L1 (gamma and beta live there).
 __device__ __forceinline__ norm_x norm_load(const row_t* p) {
+  norm_word w;
 #if NORM_BYTES == 16
-  uint4 b;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(b.x), "=r"(b.y), "=r"(b.z), "=r"(b.w) : "l"(p));
-  return b;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "l"(p));
 #else
-  return __ldcs(reinterpret_cast<const norm_x*>(p));
+  w = __ldcs(reinterpret_cast<const norm_word*>(p));
 #endif
+  norm_x r;
+  memcpy(&r, &w, NORM_BYTES);
+  return r;
+}
+// the same from shared memory
+__device__ __forceinline__ norm_x norm_shared(const norm_x* p) {
+  const norm_word w = *reinterpret_cast<const norm_word*>(p);
+  norm_x r;
+  memcpy(&r, &w, NORM_BYTES);
+  return r;
 }
 __device__ __forceinline__ void norm_wide(const norm_x& b, f32 (&v)[NORM_VE]) {
-#if NORM_BYTES == 2
-  v[0] = row_h2f(b);
-#else
-  u32 w[NORM_BYTES / 4];
+#if ROW_F16 && NORM_VE > 1
+  u32 w[NORM_VE / 2];
   memcpy(w, &b, NORM_BYTES);
 #pragma unroll
-  for (int i = 0; i < NORM_BYTES / 4; ++i) {
-#if ROW_F16
-    row_h2x2(w[i], v[2 * i], v[2 * i + 1]);
+  for (int i = 0; i < NORM_VE / 2; ++i) row_h2x2(w[i], v[2 * i], v[2 * i + 1]);
+#elif ROW_F16
+  v[0] = row_h2f(b);
 #else
-    v[i] = __uint_as_float(w[i]);
-#endif
-  }
+#pragma unroll
+  for (int e = 0; e < NORM_VE; ++e) v[e] = b.v[e];
 #endif
 }
 __device__ __forceinline__ void norm_store(row_t* p, const f32 (&v)[NORM_VE]) {
-  norm_x b;
-#if NORM_BYTES == 2
-  b = row_f2h(v[0]);
-#else
-  u32 w[NORM_BYTES / 4];
+#if ROW_F16 && NORM_VE > 1
+  u32 w[NORM_VE / 2];
 #pragma unroll
-  for (int i = 0; i < NORM_BYTES / 4; ++i) {
-#if ROW_F16
-    w[i] = row_x2h2(v[2 * i], v[2 * i + 1]);
+  for (int i = 0; i < NORM_VE / 2; ++i) w[i] = row_x2h2(v[2 * i], v[2 * i + 1]);
+#elif ROW_F16
+  const u16 w = row_f2h(v[0]);
 #else
-    w[i] = __float_as_uint(v[i]);
+  norm_x w;
+#pragma unroll
+  for (int e = 0; e < NORM_VE; ++e) w.v[e] = v[e];
 #endif
-  }
-  memcpy(&b, w, NORM_BYTES);
-#endif
-  __stcs(reinterpret_cast<norm_x*>(p), b);
+  norm_word o;
+  memcpy(&o, &w, NORM_BYTES);
+  __stcs(reinterpret_cast<norm_word*>(p), o);
 }
 // NORM_VE parameters (gamma, beta) from j on
 __device__ __forceinline__ void norm_params(const param_t* p, f32 (&v)[NORM_VE]) {
