@@ -207,30 +207,29 @@ NormShape norm_forward_shape(int64_t n, int ve, int64_t rows, int sms) {
 }
 constexpr int kNormGradElems = 16, kNormGradWarps = 16;  // gradients; twice the elements where they pass through shared memory
 // Shared memory per CTA for rows in flight: two CTAs of 256 threads per SM, or one of 512
-constexpr int64_t kRingBytes = 104 << 10, kRingBytesAlone = 208 << 10;
+constexpr int64_t kRingBytes = 112 << 10, kRingBytesAlone = 208 << 10;
+// gamma as Floats, for any length that comes to a shape
+int64_t norm_gamma_bytes(const NormShape& s) { return 4LL * s.u * s.warps * 32 * s.ve; }
 NormShape norm_grad_shape(int64_t n, int ve, int elt_bytes, int64_t rows, int sms) {
   const int bytes = ve * elt_bytes;
   // (accesses of one element: eight per lane, which leave registers for more rows at a time, as long as the row fits)
   NormShape s = norm_shape(n, ve, std::min(kNormGradElems, 8 * ve), kNormGradWarps, rows, sms);
   if (!s.whole) s = norm_shape(n, ve, kNormGradElems, kNormGradWarps, rows, sms);
   if (bytes == 2) return s;
-  int64_t rest = 0;
+  const NormShape reread = s;
   if (!s.whole) {
-    const NormShape reread = s;
     if (bytes < 16) return reread;
     s = norm_shape(n, ve, 2 * kNormGradElems, kNormGradWarps, rows, sms);
     if (!s.whole) return s;
     s.keep = false;
-    rest = 4LL * s.u * s.threads * ve;       // gamma, for any length that comes to this shape
-    if (kRingBytesAlone - rest < 2 * 2LL * bytes * s.u * s.threads) return reread;
   }
-  const int64_t stage = 2LL * bytes * s.u * s.threads, room = (s.threads > kThreads ? kRingBytesAlone : kRingBytes) - rest;
+  const int64_t stage = 2LL * bytes * s.u * s.threads, room = (s.threads > kThreads ? kRingBytesAlone : kRingBytes) - norm_gamma_bytes(s);
   s.stages = (int)std::min<int64_t>(4, room / stage);
-  return s;
+  return s.stages < 2 ? reread : s;
 }
 size_t norm_grad_smem(const NormShape& s, int elt_bytes, int64_t n) {
   if (!s.whole) return 0;
-  const size_t ring = 2u * s.ve * elt_bytes * s.u * s.threads * s.stages + (s.keep ? 0 : 4u * s.u * s.threads * s.ve), sums = s.rows() > 1 ? (size_t)n * 8 : 0;
+  const size_t ring = 2u * s.ve * elt_bytes * s.u * s.threads * s.stages + (s.stages ? norm_gamma_bytes(s) : 0), sums = s.rows() > 1 ? (size_t)n * 8 : 0;
   return std::max(ring, sums);
 }
 

@@ -8,16 +8,13 @@
 //   NORM_STAGES  rows of x and dy on their way while one is worked on: every lane copies its own elements to shared
 //                memory (cp.async) and reads them back itself, so the ring needs no barrier and no flag.  0: rows of
 //                Halves that start on odd elements (no such copy of 2 bytes exists) are loaded directly.
-//   NORM_KEEP    1: a row's blocks and gamma stay in registers between the two passes (up to 16 elements per lane);
-//                0: gamma lies in shared memory and the blocks are read from the ring twice (32 elements per lane,
-//                whose sums alone take 64 registers)
+//   NORM_KEEP    1: xh and a stay in registers between the two passes (up to 16 elements per lane); 0: the row is
+//                read from the ring twice (32 elements per lane, whose sums alone take 64 registers)
 //   NORM_LONG    rows longer than that: dx alone (x and dy read twice), the sums over rows by acc_rows_norm_cols
 
 struct Params { i64 x, gamma, mean, rstd, dy, dx, partial, dgamma, dbeta, rows, n, lines, chunk; };
 
 extern __shared__ uint4 norm_memory[];
-// gamma in registers where they suffice
-#define NORM_GAMMA_REGS (NORM_KEEP && (NORM_STAGES > 0 || NORM_U * NORM_VE <= 8))
 
 #if NORM_SUMS
 // Lines of partial sums -> dgamma, dbeta.  32 columns per CTA, the warps take lines in turn.
@@ -147,17 +144,10 @@ extern "C" __global__ void __launch_bounds__(ROW_THREADS, ROW_THREADS > 256 ? 1 
   for (int s = 0; s < NORM_STAGES - 1; ++s) fetch(row + s * stride, s);
   int stage = 0;
 #endif
-#if !NORM_KEEP
+#if NORM_STAGES
   f32* const gs = reinterpret_cast<f32*>(reinterpret_cast<norm_x*>(norm_memory) + 2 * NORM_STAGES * PLANE);
   for (int j = threadIdx.x; j < n; j += ROW_THREADS) gs[j] = row_wide(gamma[j]);
   __syncthreads();
-#elif NORM_GAMMA_REGS
-  f32 gr[NORM_U][NORM_VE];
-#pragma unroll
-  for (int u = 0; u < NORM_U; ++u) {
-    const int j = u * STEP + g * NORM_VE;
-    if (j < n) norm_params(gamma + j, gr[u]);
-  }
 #endif
   f32 mean = 0.0f, rstd = 0.0f, mean_next = 0.0f, rstd_next = 0.0f;
   if (row < p.rows) {
@@ -182,35 +172,28 @@ extern "C" __global__ void __launch_bounds__(ROW_THREADS, ROW_THREADS > 256 ? 1 
     const norm_x* const bd = mine + (2 * stage + 1) * PLANE;
     stage = (stage + 1) % NORM_STAGES;
 #endif
-#if NORM_KEEP
+#if NORM_STAGES
+#define NORM_TAKE(u)                                 \
+  norm_wide(norm_shared(bx + (u) * ROW_THREADS), v); \
+  norm_wide(norm_shared(bd + (u) * ROW_THREADS), d); \
+  norm_gamma(gs + j, ga);
+#else
     norm_x kx[NORM_U], kd[NORM_U];
 #pragma unroll
     for (int u = 0; u < NORM_U; ++u) {
       const int j = u * STEP + g * NORM_VE;
       if (there && j < n) {
-#if NORM_STAGES
-        kx[u] = norm_shared(bx + u * ROW_THREADS);
-        kd[u] = norm_shared(bd + u * ROW_THREADS);
-#else
         kx[u] = norm_load(reinterpret_cast<const row_t*>(p.x) + row * p.n + j);
         kd[u] = norm_load(reinterpret_cast<const row_t*>(p.dy) + row * p.n + j);
-#endif
       }
     }
-#if NORM_GAMMA_REGS
-#define NORM_GAMMA(u) for (int e = 0; e < NORM_VE; ++e) ga[e] = gr[u][e];
-#else
-#define NORM_GAMMA(u) norm_params(gamma + j, ga);     // (from L1: these lanes need their registers)
+#define NORM_TAKE(u)   \
+  norm_wide(kx[u], v); \
+  norm_wide(kd[u], d); \
+  norm_params(gamma + j, ga);
 #endif
-#define NORM_TAKE(u)     \
-  norm_wide(kx[u], v);   \
-  norm_wide(kd[u], d);   \
-  NORM_GAMMA(u)
-#else
-#define NORM_TAKE(u)                                 \
-  norm_wide(norm_shared(bx + (u) * ROW_THREADS), v); \
-  norm_wide(norm_shared(bd + (u) * ROW_THREADS), d); \
-  norm_gamma(gs + j, ga);
+#if NORM_KEEP
+    f32 xh_kept[NORM_U][NORM_VE], a_kept[NORM_U][NORM_VE];
 #endif
     f32 s[2] = {0.0f, 0.0f};
 #pragma unroll
@@ -226,6 +209,10 @@ extern "C" __global__ void __launch_bounds__(ROW_THREADS, ROW_THREADS > 256 ? 1 
           s[1] = fmaf(a, xh, s[1]);
           sg[u * NORM_VE + e] = fmaf(d[e], xh, sg[u * NORM_VE + e]);
           sb[u * NORM_VE + e] += d[e];
+#if NORM_KEEP
+          xh_kept[u][e] = xh;
+          a_kept[u][e] = a;
+#endif
         }
       }
     }
@@ -237,10 +224,16 @@ extern "C" __global__ void __launch_bounds__(ROW_THREADS, ROW_THREADS > 256 ? 1 
     for (int u = 0; u < NORM_U; ++u) {
       const int j = u * STEP + g * NORM_VE;
       if (there && j < n) {
-        f32 v[NORM_VE], d[NORM_VE], ga[NORM_VE];
+        f32 v[NORM_VE];
+#if NORM_KEEP
+#pragma unroll
+        for (int e = 0; e < NORM_VE; ++e) v[e] = rstd * fmaf(-xh_kept[u][e], mb, a_kept[u][e] - ma);
+#else
+        f32 d[NORM_VE], ga[NORM_VE];
         NORM_TAKE(u)
 #pragma unroll
-        for (int e = 0; e < NORM_VE; ++e) v[e] = rstd * (fmaf(-((v[e] - mean) * rstd), mb, fmaf(d[e], ga[e], -ma)));
+        for (int e = 0; e < NORM_VE; ++e) v[e] = rstd * fmaf(-((v[e] - mean) * rstd), mb, d[e] * ga[e] - ma);
+#endif
         norm_store(dx + j, v);
       }
     }
