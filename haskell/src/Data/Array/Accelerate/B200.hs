@@ -35,6 +35,7 @@ module Data.Array.Accelerate.B200 (
   B200, createB200, defaultB200,
   run, run1, runN,
   runWith, runNWith,
+  B200Foreign(..),
 ) where
 
 import Data.Array.Accelerate.AST
@@ -56,12 +57,14 @@ import Data.Array.Accelerate.Trafo.Sharing                          ( Afunction(
 import Data.Array.Accelerate.Type
 import qualified Data.Array.Accelerate.Smart                        as Smart
 import qualified Data.Array.Accelerate.Sugar.Array                  as Sugar
+import Data.Array.Accelerate.Sugar.Foreign                          ( Foreign(..) )
 
 import Control.Exception                                            ( throwIO, ErrorCall(..), ArithException(..) )
 import Control.Monad
 import Data.Int
 import Data.IORef
 import Data.List                                                    ( intercalate )
+import Data.Typeable                                                ( Typeable, (:~:)(..), eqT )
 import Data.Word
 import Foreign.C.String
 import Foreign.C.Types
@@ -74,6 +77,25 @@ import qualified Data.ByteString                                    as B
 import qualified Data.Text                                          as T
 import qualified Data.Text.Encoding                                 as T
 import System.IO.Unsafe                                             ( unsafePerformIO )
+
+
+-- Foreign array functions ------------------------------------------------------
+
+-- | A kernel of the library behind an array function, by name and constants, for
+-- @foreignAcc@: @foreignAcc (B200Foreign "b200.layerNorm" [1e-5]) definition@.  The
+-- names, with their constants, arguments and results, are listed at the head of
+-- @accelerate_b200/csrc/rows.cpp@; the definitions in array code that belong to
+-- them are those of @accelerate_b200/rows.py@.
+data B200Foreign f where
+  B200Foreign :: String -> [Double] -> B200Foreign (as -> bs)
+
+instance Foreign B200Foreign where
+  strForeign (B200Foreign name _) = name
+
+b200Foreign :: forall asm as bs. Typeable asm => asm (as -> bs) -> Maybe (String, [Double])
+b200Foreign asm = case eqT :: Maybe (asm :~: B200Foreign) of
+  Just Refl | B200Foreign name cs <- asm -> Just (name, cs)
+  _                                      -> Nothing
 
 
 -- C ABI (include/accelerate_b200.h) ------------------------------------------
@@ -301,6 +323,7 @@ unsupported what = error ("accelerate-b200: " ++ what ++ " are not supported by 
 --            | (use (array RANK ELT) (shape d..) (hex BYTES)+)        -- Use: one (hex ..) per scalar leaf
 --            | (acond exp (branch BODY) (branch BODY))                 -- Acond
 --            | (awhile AFUN AFUN (args NAME*)) | (apply AFUN (args NAME*))
+--            | (aforeign NAME (consts NUMBER*) AFUN (args NAME*))      -- Aforeign with a kernel of this backend
 --            | (atrace (hex MESSAGE) (show NAME*) (args NAME*))        -- Atrace: print, then hand the args on
 --   AFUN    := (afun ((NAME (array RANK ELT))*) BODY)
 --   BODY    := (let LHS NODE)* (out NAME+)
@@ -417,11 +440,13 @@ nodeText pacc ns s = case pacc of
   Apply _ f a                  -> let (xs, s1) = manifestArrays a ns s
                                       (fb, s2) = afunText f ns s1
                                   in  (sx ["apply", fb, sx ("args" : xs)], s2)
-  -- no foreign implementation is registered for this backend: the pure fallback runs, as in the
-  -- interpreter (Interpreter.hs:217)
-  Aforeign _ _ f a             -> let (xs, s1) = manifestArrays a ns s
+  -- a function the library has a kernel for goes by its name; of other backends' functions the pure
+  -- definition runs, as in the interpreter (Interpreter.hs:217)
+  Aforeign _ asm f a           -> let (xs, s1) = manifestArrays a ns s
                                       (fb, s2) = afunText f ns s1
-                                  in  (sx ["apply", fb, sx ("args" : xs)], s2)
+                                  in  case b200Foreign asm of
+                                        Just (name, cs) -> (sx ["aforeign", name, sx ("consts" : map (`showHFloat` "") cs), fb, sx ("args" : xs)], s2)
+                                        Nothing         -> (sx ["apply", fb, sx ("args" : xs)], s2)
   -- Interpreter.hs:215: the library prints the message and its own rendering of the arrays (the
   -- Message's `show` is a Haskell closure and stays on this side of the boundary)
   Atrace (Message _ _ msg) a b -> let (xs, s1) = manifestArrays a ns s

@@ -107,7 +107,15 @@ int b200_array_devptr(b200_ctx* ctx, uint64_t id, int leaf, void** ptr);
  * i.e. what Interpreter.runN obtains from convertAfun (Interpreter.hs:110-118).
  * Parses, type-checks and generates the kernels' scalar code; kernels are
  * compiled by NVRTC on first use and cached by content hash (in memory and in
- * $ACCELERATE_B200_CACHE_DIR). */
+ * $ACCELERATE_B200_CACHE_DIR).
+ * A foreign array function (Aforeign, AST.hs:307-316) is (aforeign NAME (consts c..) AFUN (args a..)); AFUN is its
+ * definition in array code.  Behind these names the library has kernels, and AFUN only gives the result's type:
+ * b200.logProbs, b200.distill, b200.distillGrad, b200.layerNorm, b200.layerNormGrad (log probabilities with entropy and
+ * top alternatives, distillation from a teacher's top logits, layer norm; Half or Float rows).  Their constants and
+ * arguments are checked here (B200_ERR_TYPE, B200_ERR_ARG, B200_ERR_UNSUPPORTED) and their shapes by the run
+ * (B200_ERR_BOUNDS, "shape mismatch"); a token or id behind its row's end is reported like any index out of bounds, by the
+ * next download or b200_sync.  They cannot be captured into a CUDA graph (B200_ERR_UNSUPPORTED): their results come from
+ * the context's pool.  Any other NAME: AFUN is applied (Interpreter.hs:217). */
 int b200_program_load(b200_ctx* ctx, const char* text, size_t len, b200_program** out);
 void b200_program_free(b200_program* prog);
 int b200_program_num_inputs(b200_program* prog, int* n);
