@@ -126,6 +126,7 @@ def kernel_source(text, node=0):
 
 
 _LEAVES, _ELT_TEXT = {}, {}
+_SCALAR_TEXT = {t: t.encode() for t in L.SCALARS}
 
 
 def _leaf_types(elt):
@@ -155,9 +156,10 @@ class DeviceArray:
 
     def __init__(self, ctx, ident, elt=None, shape=None, leaf_types=None, ptrs=None):
         self.ctx, self.id, self._ptrs = ctx, ident, ptrs
-        if shape is not None and (elt is not None or leaf_types is not None):
-            self.shape = shape
-            self.leaf_types = leaf_types if leaf_types is not None else list(_leaf_types(elt))
+        if leaf_types is not None:
+            self.shape, self.leaf_types = shape, leaf_types
+        elif shape is not None and elt is not None:
+            self.shape, self.leaf_types = shape, list(_leaf_types(elt))
         else:
             rank, leaves = ctypes.c_int(), ctypes.c_int()
             for most_rank, most_leaves in ((8, 32), (1 << 10, 1 << 16)):
@@ -219,8 +221,10 @@ class DeviceArray:
             self.id = self._ptrs = None
 
     def __del__(self):
+        # (free() without its frame: every temporary array comes through here)
         try:
-            self.free()
+            if self.id is not None and self.ctx.handle:
+                _fast.free(self.ctx.handle, self.id)
         except Exception:
             pass
 
@@ -290,6 +294,10 @@ class Context:
     def forget(self, key):
         _check(lib().b200_array_forget(self.h, key))
         self._interned.pop(key, None)
+
+    def wrap_scalars(self, elt, shape, ptr):
+        """``wrap`` for a scalar element type and a tuple of ints as the shape."""
+        return DeviceArray(self, _fast.wrap(self.handle, _SCALAR_TEXT[elt], shape, (ptr,)), elt, shape, [elt])
 
     def wrap(self, elt, shape, ptrs):
         """Adopt caller-owned device memory (one pointer per leaf)."""

@@ -45,6 +45,8 @@ bool mentions_vector(const Type& t) {
 // element type of an array the caller creates.  SIMD vectors have no array type of their own here: an
 // `Array sh (Vec n t)` is created as an array of t of shape sh :. n, the same bytes (Array/Data.hs:108-119).
 Type parse_type_text(const char* s) {
+  for (int k = 0; k < NTY; ++k)
+    if (!strcmp(s, ty_name[k])) return Type::scalar((Ty)k);
   Sx x = parse_sexp(s, strlen(s));
   Type t = parse_type(x);
   if (mentions_vector(t)) throw Error(B200_ERR_TYPE, "an array of (vec n t) is created as an array of t with one more, innermost, dimension of extent n");

@@ -90,6 +90,7 @@ class _View:
         self.__cuda_array_interface__ = {"shape": shape, "typestr": typestr, "data": (ptr, False), "version": 3}
 
 
+_as_tensor = torch.as_tensor
 _TYPESTR = {t: np.dtype(d).str for t, d in L.NP_OF.items()}
 
 
@@ -147,7 +148,7 @@ class GpuExecutor:
         if 0 in shape:
             dt = np.dtype(L.NP_OF[a.leaf_types[leaf]])
             return torch.empty(a.shape, dtype=torch.from_numpy(np.empty(0, dt)).dtype, device=self.stream.device)
-        t = torch.as_tensor(_View(shape or (1,), _TYPESTR[a.leaf_types[leaf]], a.devptr(leaf)), device=self.device)
+        t = _as_tensor(_View(shape or (1,), _TYPESTR[a.leaf_types[leaf]], a.devptr(leaf)), device=self.device)
         t._keepalive = a
         return t
 
@@ -156,7 +157,7 @@ class GpuExecutor:
         must be contiguous."""
         if not t.is_contiguous():
             raise ValueError("only a contiguous tensor can be an array's memory")
-        a = self.ctx.wrap(elt, tuple(t.shape), [t.data_ptr()])
+        a = self.ctx.wrap_scalars(elt, tuple(t.shape), t.data_ptr()) if isinstance(elt, str) and elt in L.NP_OF else self.ctx.wrap(elt, tuple(t.shape), [t.data_ptr()])
         a._keepalive = t
         return a
 
