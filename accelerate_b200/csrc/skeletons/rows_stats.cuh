@@ -110,12 +110,21 @@ template <int Q> __device__ __forceinline__ void st_rank(int sorted, int n, int 
         rank[q] = lo;
       }
     }
-#pragma unroll 4
-    for (int i = sorted; i < n; ++i) {
-      const u64 c = sh.cand[i];
+    int i = sorted;
+    if ((i & 1) && i < n) {
 #pragma unroll
-      for (int q = 0; q < Q; ++q) rank[q] += c > key[q];
+      for (int q = 0; q < Q; ++q) rank[q] += sh.cand[i] > key[q];
+      ++i;
     }
+#pragma unroll 4
+    for (; i + 1 < n; i += 2) {
+      const ulonglong2 c = *reinterpret_cast<const ulonglong2*>(&sh.cand[i]);
+#pragma unroll
+      for (int q = 0; q < Q; ++q) rank[q] += (c.x > key[q]) + (c.y > key[q]);
+    }
+    if (i < n)
+#pragma unroll
+      for (int q = 0; q < Q; ++q) rank[q] += sh.cand[i] > key[q];
   }
   __syncthreads();
 #pragma unroll
@@ -124,11 +133,30 @@ template <int Q> __device__ __forceinline__ void st_rank(int sorted, int n, int 
   if (tid == 0) sh.count = n < k ? n : k;
   __syncthreads();
 }
+// The same for so few candidates that 2^SPLIT threads can share the counting for each: what a drain waits for is the
+// length of that loop.
+template <int SPLIT> __device__ __forceinline__ void st_rank_few(int n, int k) {
+  const int tid = threadIdx.x, i = tid >> SPLIT;
+  const u64 key = i < n ? sh.cand[i] : 0;
+  int rank = 0;
+#pragma unroll 4
+  for (int j = tid & ((1 << SPLIT) - 1); j < n; j += 1 << SPLIT) rank += sh.cand[j] > key;
+#pragma unroll
+  for (int d = 1; d < (1 << SPLIT); d <<= 1) rank += __shfl_xor_sync(ACC_FULL_MASK, rank, d);
+  __syncthreads();
+  if (i < n && (tid & ((1 << SPLIT) - 1)) == 0 && rank < k) sh.cand[rank] = key;
+  if (tid == 0) sh.count = n < k ? n : k;
+  __syncthreads();
+}
 // The best k of the n candidates, in falling order, to the front of the list, and their number.  Long lists
 // (rows in an unusual order): a bitonic sort.
 __device__ __forceinline__ int st_compact(int sorted, int n, int k) {
   const int tid = threadIdx.x;
-  if (n <= ROW_THREADS) {
+  if (n <= ROW_THREADS / 4) {
+    st_rank_few<2>(n, k);
+  } else if (n <= ROW_THREADS / 2) {
+    st_rank_few<1>(n, k);
+  } else if (n <= ROW_THREADS) {
     st_rank<1>(sorted, n, k);
   } else if (n <= 2 * ROW_THREADS) {
     st_rank<2>(sorted, n, k);
