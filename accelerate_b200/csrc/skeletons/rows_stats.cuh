@@ -40,7 +40,6 @@ struct st_shared {
   int warp_count[ST_WARPS];
 };
 
-
 extern __shared__ uint4 st_memory[];
 static_assert(sizeof(st_shared) <= ROW_SMEM, "the host asks for less shared memory than the kernel uses");
 #define sh (*reinterpret_cast<st_shared*>(st_memory))

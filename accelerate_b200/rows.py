@@ -166,7 +166,7 @@ def distill(tau, ids, teacher, student):
 
     ``distill :: Float -> Array (sh:.Int) Int32 -> Array (sh:.Int) t' -> Array (sh:.Int) t -> (Array sh Float, Array sh Float)``
 
-    ``ids`` and ``teacher`` hold a few tokens per row and the teacher's logits (or log probabilities) for them, as
+    ``ids`` and ``teacher`` hold a few tokens per row (at most 4096) and the teacher's logits (or log probabilities) for them, as
     ``logProbs`` yields them.  With q the softmax of teacher / tau over the entries and p that of student / tau over the
     whole row, the loss is tau^2 sum q (ln q - ln p).  The second result is ln sum e^(student / tau), which
     ``distillGrad`` takes.

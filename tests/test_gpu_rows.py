@@ -115,7 +115,7 @@ def test_rows_agree_with_the_definitions(gpu_ctx):
 
 @pytest.mark.parametrize("t,tt", [("f16", "f32"), ("f16", "f16"), ("f32", "f32"), ("f32", "f16")])
 @pytest.mark.parametrize("rows,n,k,tau", [(1, 1, 1, 1.0), (3, 50, 7, 2.0), (5, 1000, 1, 0.5), (2, 4097, 33, 1.0), (700, 300, 20, 4.0), (1, 131072, 64, 2.0), (4, 50257, 100, 1.0),
-                                          (2, 2000, 600, 1.5)])
+                                          (2, 2000, 600, 1.5), (2, 9000, 4096, 1.0)])
 def test_distill_and_its_gradient(gpu_ctx, t, tt, rows, n, k, tau):
     g = G(rows + n + k)
     x = R.logits(g, (rows, n), t)
@@ -299,6 +299,15 @@ def test_a_capture_is_refused(gpu_ctx):
     assert e.value.code == 6 and "captured" in str(e.value)
     y, _ = gpu_ctx.execute(prog.text, [v, v, x], 2)
     assert np.array_equal(y.download(), np.ones((2, 8), np.float32))
+
+
+def test_too_many_teacher_entries_are_refused(gpu_ctx):
+    x, ids, te = np.zeros((1, 5000), np.float32), np.zeros((1, 4097), np.int32), np.zeros((1, 4097), np.float32)
+    one = np.ones(1, np.float32)
+    for term in (A.distill(1.0, ids, te, x), [A.distillGrad(1.0, ids, te, x, one, one)]):
+        with pytest.raises(backend.B200Error) as e:
+            RUN(term)
+        assert e.value.code == 6 and "4096" in str(e.value)
 
 
 def test_memory_that_cannot_be_an_array_is_refused(gpu_ctx):
