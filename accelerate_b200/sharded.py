@@ -86,9 +86,6 @@ class _View:
 
     __slots__ = ("__cuda_array_interface__",)
 
-    def __init__(self, shape, typestr, ptr):
-        self.__cuda_array_interface__ = {"shape": shape, "typestr": typestr, "data": (ptr, False), "version": 3}
-
 
 _as_tensor = torch.as_tensor
 _TYPESTR = {t: np.dtype(d).str for t, d in L.NP_OF.items()}
@@ -148,7 +145,9 @@ class GpuExecutor:
         if 0 in shape:
             dt = np.dtype(L.NP_OF[a.leaf_types[leaf]])
             return torch.empty(a.shape, dtype=torch.from_numpy(np.empty(0, dt)).dtype, device=self.stream.device)
-        t = _as_tensor(_View(shape or (1,), _TYPESTR[a.leaf_types[leaf]], a.devptr(leaf)), device=self.device)
+        v = _View()
+        v.__cuda_array_interface__ = {"shape": shape or (1,), "typestr": _TYPESTR[a.leaf_types[leaf]], "data": (a.devptr(leaf), False), "version": 3}
+        t = _as_tensor(v, device=self.device)
         t._keepalive = a
         return t
 
