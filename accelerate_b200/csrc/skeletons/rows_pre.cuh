@@ -31,6 +31,15 @@ __device__ __forceinline__ void row_h2x2(u32 w, f32& lo, f32& hi) {
 }
 __device__ __forceinline__ u32 row_x2h2(f32 lo, f32 hi) { u32 r; asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo)); return r; }
 
+// Two Floats in one 64-bit register: an instruction does both (each rounded as if alone).  The row kernels are near
+// the limit of instructions issued, not of arithmetic, so this is what it saves: half the additions' and products' slots.
+typedef u64 row_two;
+__device__ __forceinline__ row_two row_pair(f32 a, f32 b) { row_two r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b)); return r; }
+__device__ __forceinline__ void row_split(row_two v, f32& a, f32& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ row_two row_fma2(row_two a, row_two b, row_two c) { row_two r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
+__device__ __forceinline__ row_two row_mul2(row_two a, row_two b) { row_two r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ __forceinline__ row_two row_add2(row_two a, row_two b) { row_two r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+
 // The elements of a 16-byte block as Floats, and back (rounded to nearest even).
 __device__ __forceinline__ void row_unpack(const uint4& b, f32 (&v)[ROW_E]) {
   const u32 w[4] = {b.x, b.y, b.z, b.w};

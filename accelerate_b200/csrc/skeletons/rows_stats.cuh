@@ -374,33 +374,40 @@ acc_rows_stats(const __grid_constant__ Params p) {
       }
       st.m = mn;
     }
+    const row_two cc = row_pair(c, c);
 #if ROW_F16
     const f32 neg = -(st_base(st.m) * c);
-#define ST_T(x) fmaf(x, c, neg)
+    const row_two nn = row_pair(neg, neg);
+#define ST_T(x) row_fma2(x, cc, nn)
 #else
-    const f32 base = st_base(st.m);
-#define ST_T(x) (((x) - base) * c)
+    const f32 neg = -st_base(st.m);
+    const row_two nn = row_pair(neg, neg);
+#define ST_T(x) row_mul2(row_add2(x, nn), cc)
 #endif
-    f32 z0 = 0.0f, z1 = 0.0f, w0 = 0.0f, w1 = 0.0f;
+    row_two z0 = 0, z1 = 0, w0 = 0, w1 = 0;          // (pairs of +0)
 #pragma unroll
     for (int u = 0; u < ROW_U; ++u) {
       f32 v[ROW_E];
       row_unpack(cur[u], v);
 #pragma unroll
       for (int e = 0; e < ROW_E; e += 2) {
-        const f32 ta = ST_T(v[e]), tb = ST_T(v[e + 1]);
-        const f32 ea = row_ex2(ta), eb = row_ex2(tb);
-        z0 += ea;
-        z1 += eb;
+        f32 ta, tb;
+        row_split(ST_T(row_pair(v[e], v[e + 1])), ta, tb);
+        const row_two ex = row_pair(row_ex2(ta), row_ex2(tb));
+        row_two& z = e & 2 ? z1 : z0;
+        z = row_add2(z, ex);
 #if !ROW_DISTILL
         // (a masked element has t = -inf and 2^t = 0: the bound keeps their product at 0)
-        w0 = fmaf(ea, fmaxf(ta, -1000.0f), w0);
-        w1 = fmaf(eb, fmaxf(tb, -1000.0f), w1);
+        row_two& w = e & 2 ? w1 : w0;
+        w = row_fma2(ex, row_pair(fmaxf(ta, -1000.0f), fmaxf(tb, -1000.0f)), w);
 #endif
       }
     }
-    st.z += z0 + z1;
-    st.w += w0 + w1;
+    f32 za, zb, wa, wb;
+    row_split(row_add2(z0, z1), za, zb);
+    row_split(row_add2(w0, w1), wa, wb);
+    st.z += za + zb;
+    st.w += wa + wb;
 
 #if ROW_TOPK
     // The list is drained behind the first tile and whenever the part of the row seen since has doubled: each time
