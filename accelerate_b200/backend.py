@@ -155,7 +155,7 @@ class DeviceArray:
     shape passes both; otherwise the library is asked, once."""
 
     def __init__(self, ctx, ident, elt=None, shape=None, leaf_types=None, ptrs=None):
-        self.ctx, self.id, self._ptrs = ctx, ident, ptrs
+        self.ctx, self.id, self._ptrs, self._since = ctx, ident, ptrs, ctx.adoptions
         if leaf_types is not None:
             self.shape, self.leaf_types = shape, leaf_types
         elif shape is not None and elt is not None:
@@ -173,7 +173,9 @@ class DeviceArray:
         self.elt = elt if elt is not None else (self.leaf_types[0] if len(self.leaf_types) == 1 else tuple(self.leaf_types))
 
     def devptr(self, leaf=0):
-        if self._ptrs is not None and 0 <= leaf < len(self._ptrs):
+        # (the pointers a run reported hold as long as no payload was adopted since: this may be a second handle of the
+        # array that adopted it, and the library copies the payload when it is asked for the pointer)
+        if self._ptrs is not None and 0 <= leaf < len(self._ptrs) and self._since == self.ctx.adoptions:
             return self._ptrs[leaf]
         p = ctypes.c_void_p()
         _check(lib().b200_array_devptr(self.ctx.h, self.id, leaf, ctypes.byref(p)))
@@ -188,10 +190,12 @@ class DeviceArray:
     def adopt_host(self, leaves):
         """Lazy upload: the host arrays are copied when the array is first used on the device;
         they are kept alive by this object until then."""
-        self._ptrs = None                # (the library copies the payload when it is next asked for the pointer)
         self._adopted = [np.ascontiguousarray(a) for a in leaves]
-        for k, a in enumerate(self._adopted):
-            _check(lib().b200_array_adopt_host(self.ctx.h, self.id, k, a.ctypes.data, a.nbytes))
+        try:
+            for k, a in enumerate(self._adopted):
+                _check(lib().b200_array_adopt_host(self.ctx.h, self.id, k, a.ctypes.data, a.nbytes))
+        finally:
+            self.ctx.adoptions += 1
         return self
 
     def download(self, out=None):
@@ -240,6 +244,7 @@ class Context:
         self._programs = {}
         self._inflight = []          # views with an asynchronous download under way (kept alive until sync)
         self._interned = {}          # host payloads registered in the memory table, by key
+        self.adoptions = 0           # payloads adopted so far (DeviceArray.devptr)
 
     def close(self):
         if self.h:

@@ -1,0 +1,64 @@
+"""The Python layer's calls into the library, without a GPU: a library that records and answers stands in for it."""
+import ctypes
+
+import numpy as np
+import pytest
+
+from accelerate_b200 import backend
+
+
+class Library:
+    """Every entry point succeeds; `devptr` answers with `now`."""
+
+    now = 0
+
+    def __getattr__(self, name):
+        return lambda *a: 0
+
+    def b200_array_devptr(self, ctx, ident, leaf, out):
+        ctypes.cast(out, ctypes.POINTER(ctypes.c_void_p))[0] = self.now
+        return 0
+
+
+class Fast:
+    """The compiled binding: a run yields one vector of two Floats at `now`."""
+
+    def __init__(self, library):
+        self.library, self.wrapped = library, []
+
+    def execute(self, ctx, prog, ids, n_out):
+        return [(9, (2,), ["f32"], (self.library.now,))]
+
+    def wrap(self, ctx, elt, shape, ptrs):
+        self.wrapped.append((elt, tuple(shape), tuple(ptrs)))
+        return 10
+
+    def free(self, ctx, ident):
+        return 0
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    library = Library()
+    fast = Fast(library)
+    monkeypatch.setattr(backend, "lib", lambda: library)
+    monkeypatch.setattr(backend, "_fast", fast)
+    ctx = backend.Context(0)
+    ctx._programs["p"] = ctypes.c_void_p(1)
+    return ctx, library, fast
+
+
+def test_a_result_that_is_an_input_asks_again_once_the_input_was_given_other_data(calls):
+    """A program may hand an input on as its result: two handles of one array.  A payload adopted through one of them is
+    copied when the array's pointer is next asked for, through either."""
+    ctx, library, _ = calls
+    a = ctx.array("f32", (2,))
+    library.now = 111
+    out, = ctx.execute("p", [a], 1)
+    assert out.devptr() == 111
+    a.adopt_host([np.ones(2, np.float32)])
+    library.now = 222
+    assert out.devptr() == 222, "the library was not asked, and the adopted payload stays where it is"
+    after, = ctx.execute("p", [a], 1)
+    library.now = 333
+    assert after.devptr() == 222, "known from the run"
