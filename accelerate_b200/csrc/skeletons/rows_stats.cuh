@@ -6,7 +6,9 @@
 // Mathematics.  With c = log2(e)/tau and m the running maximum, every thread keeps Z = sum 2^t and
 // W = sum 2^t t over its elements, t = c (x - m), and moves both to a new maximum m' by Z' = s Z,
 // W' = s (W + d Z), d = c (m - m'), s = 2^d.  Threads, warps and CTAs join by the same rule.  Then
-//   lse = m/tau + ln Z,     entropy = ln Z - ln 2 W / Z.
+//   lse = m/tau + ln Z,     entropy = ln Z - ln 2 W / Z,     ln p_j = (x_j - m)/tau - ln Z.
+// (not x_j/tau - lse: one Float holds lse to half a step of its own size, which for a row around 1e6 is 0.03, and a row
+// of nothing but the type's lowest value would come out with a probability of 1 for each of its elements)
 // Half: t = c x - M with M = c m rounded, one instruction; what the rounding shifts is known exactly and comes
 // off the end (M - c m).  Float: the subtraction first, since c m can leave the range (rows masked with the
 // type's lowest value); a Float element has twice the bytes to pay for the second instruction.
@@ -493,17 +495,19 @@ acc_rows_stats(const __grid_constant__ Params p) {
 #endif
 
   // a row without an element above -inf has no distribution: its normaliser is -inf
-  f32 lse = -ROW_INF;
-  if (st.m != -ROW_INF || st.z != 0.0f) {
-    lse = st_base(st.m) / tau + logf(st.z);
+  const bool none = st.m == -ROW_INF && st.z == 0.0f;
+  const f32 base = st_base(st.m);
+  f32 ln_z = -ROW_INF;                   // ln sum e^((x - m) / tau)
+  if (!none) {
+    ln_z = logf(st.z);
 #if ROW_F16
-    const f32 base = st_base(st.m);
-    lse += ROW_LN2 * fmaf(-base, c, base * c);
+    ln_z += ROW_LN2 * fmaf(-base, c, base * c);
 #endif
   }
+  const f32 lse = base / tau + ln_z;
 #if ROW_DISTILL
   // The teacher's entries, one warp: with e_i = exp((t_i - max t)/tau) and E their sum, q_i = e_i / E and
-  // loss = tau^2 (sum e_i ((t_i - max t) - s_i) / (tau E) - ln E + lse).
+  // loss = tau^2 (sum e_i ((t_i - max t) - (s_i - m)) / (tau E) - ln E + ln Z).
   if (warp == 0) {
     const i32* ids = reinterpret_cast<const i32*>(p.tok) + row * p.k;
     const teacher_t* ts = reinterpret_cast<const teacher_t*>(p.teacher) + row * p.k;
@@ -524,7 +528,7 @@ acc_rows_stats(const __grid_constant__ Params p) {
         const f32 e = row_ex2(dt * c);
         if (e != 0.0f) {
           es += e;
-          as += e * ((dt - row_wide(span.x[id])) / tau);
+          as += e * ((dt - (row_wide(span.x[id]) - base)) / tau);
         }
       }
     }
@@ -533,7 +537,7 @@ acc_rows_stats(const __grid_constant__ Params p) {
     bad = __any_sync(ACC_FULL_MASK, bad);
     if (lane == 0) {
       f32 loss = 0.0f;                   // no entry, no loss
-      if (es != 0.0f) loss = lse == -ROW_INF ? ROW_INF : tau * tau * (as / es - logf(es) + lse);
+      if (es != 0.0f) loss = none ? ROW_INF : tau * tau * (as / es - logf(es) + ln_z);
       if (bad) {
         acc_fail(p.err, 1003);           // "index out of bounds", reported by the next download or b200_sync
         loss = ROW_NAN;
@@ -550,11 +554,11 @@ acc_rows_stats(const __grid_constant__ Params p) {
       acc_fail(p.err, 1003);
       logp = ROW_NAN;
     } else if (tok >= 0) {
-      logp = lse == -ROW_INF ? -ROW_INF : row_wide(span.x[tok]) - lse;
+      logp = none ? -ROW_INF : row_wide(span.x[tok]) - base - ln_z;
     }
     reinterpret_cast<f32*>(p.out0)[row] = logp;
     reinterpret_cast<f32*>(p.out1)[row] = lse;
-    reinterpret_cast<f32*>(p.out2)[row] = lse == -ROW_INF ? 0.0f : logf(st.z) - ROW_LN2 * (st.w / st.z);
+    reinterpret_cast<f32*>(p.out2)[row] = none ? 0.0f : logf(st.z) - ROW_LN2 * (st.w / st.z);
   }
 #if ROW_TOPK
   __syncthreads();
@@ -586,7 +590,7 @@ acc_rows_stats(const __grid_constant__ Params p) {
     if (tid < held) {
       const u64 key = sh.cand[tid];
       id = st_index(key);
-      if (lse != -ROW_INF) logp = st_value((u32)(key >> 32)) - lse;
+      if (!none) logp = st_value((u32)(key >> 32)) - base - ln_z;
     }
     reinterpret_cast<i32*>(p.out3)[row * p.k + tid] = id;
     reinterpret_cast<f32*>(p.out4)[row * p.k + tid] = logp;

@@ -67,7 +67,8 @@ _add = lambda a, b: a + b  # noqa: E731
 
 
 def _normaliser(tau, xs):
-    """ln sum e^(x / tau) of every row, its maximum (0 for a row without an element above -inf), and the sum."""
+    """ln sum e^(x / tau) of every row, its maximum m (0 for a row without an element above -inf), and
+    z = sum e^((x - m) / tau) (0 for such a row)."""
     r = xs.rank
     m = compute(map_(lambda v: cond(v.eq(_f(-math.inf)), _f(0), v), fold(max_, _f(-math.inf), map_(_wide, xs))))
     z = compute(fold(_add, _f(0), generate(xs.shape, lambda ix: exp((_wide(xs[ix]) - m[_outer(ix, r)]) / _f(tau)))))
@@ -75,9 +76,10 @@ def _normaliser(tau, xs):
     return lse, m, z
 
 
-def _log_probability(x, lse):
-    """x - lse; a row without an element above -inf gives none of its elements any probability."""
-    return cond(lse.eq(_f(-math.inf)), _f(-math.inf), x - lse)
+def _log_probability(x, tau, m, z):
+    """(x - m) / tau - ln z: the differences inside the row, whatever its elements' size (the normaliser, one Float, has
+    lost them at 1e8).  A row without an element above -inf gives none of its elements any probability."""
+    return cond(z.eq(_f(0)), _f(-math.inf), (x - m) / _f(tau) - log(z))
 
 
 def _better(a, b):
@@ -95,7 +97,8 @@ def logProbs(k, tokens, logits):
 
     For a row x with lse = ln sum e^x the first result holds (x_token - lse, lse, entropy), the second the indices and
     log probabilities of the k largest logits, in falling order, equal ones by rising index.  k goes from 0 to 128;
-    tokens may be Int32 or Int.
+    tokens may be Int32 or Int.  Log probabilities come from the distances to the row's largest logit, not from the rounded
+    lse: they are as good for logits around 1e8 as around 0.
 
     A negative token is no token: its log probability is 0.  A token behind the row's end is an error ("index out of
     bounds", reported by the next download or sync).  Logits of -inf are masked: probability 0, and no part of the entropy.  A row
@@ -119,8 +122,8 @@ def logProbs(k, tokens, logits):
 
         def stats(o):
             t = from_integral(tok[o], INT)
-            logp = cond(t < 0, _f(0), _log_probability(_wide(xs[_inner(o, r, t)]), lse[o]))
-            return tup(logp, lse[o], cond(lse[o].eq(_f(-math.inf)), _f(0), log(z[o]) - w[o] / z[o]))
+            logp = cond(t < 0, _f(0), _log_probability(_wide(xs[_inner(o, r, t)]), 1.0, m[o], z[o]))
+            return tup(logp, lse[o], cond(z[o].eq(_f(0)), _f(0), log(z[o]) - w[o] / z[o]))
         best, last = [], None
         for _ in range(k):
             # the best element behind the one before it in the order
@@ -136,7 +139,7 @@ def logProbs(k, tokens, logits):
             for j in reversed(range(k)):
                 e = cond(ix[r - 1].eq(lift(j, INT)), best[j][o], e)
             there = e[1].ne(constant(_NONE, "i32"))
-            return tup(cond(there, e[1], constant(-1, "i32")), cond(there, _log_probability(e[0], lse[o]), _f(-math.inf)))
+            return tup(cond(there, e[1], constant(-1, "i32")), cond(there, _log_probability(e[0], 1.0, m[o], z[o]), _f(-math.inf)))
         outer = _outer(xs.shape, r)
         return generate(outer, stats), generate(_inner(outer, r, lift(k, INT)), alternative)
     return _foreign("b200.logProbs", [k], definition, tokens, logits)
@@ -179,13 +182,13 @@ def distill(tau, ids, teacher, student):
 
     def definition(ids, ts, xs):
         r = xs.rank
-        lse, _, _ = _normaliser(tau, xs)
+        lse, top, z = _normaliser(tau, xs)
         m, total, e = _teacher(tau, ids, ts)
 
         def term(ix):
             o = _outer(ix, r)
             w = e(ix) / total[o]
-            lp = _log_probability(_wide(xs[_inner(o, r, from_integral(ids[ix], INT))]) / _f(tau), lse[o])
+            lp = _log_probability(_wide(xs[_inner(o, r, from_integral(ids[ix], INT))]), tau, top[o], z[o])
             return cond(ids[ix] < constant(0, "i32"), _f(0),
                         cond(e(ix).eq(_f(0)), _f(0), w * ((_wide(ts[ix]) - m[o]) / _f(tau) - log(total[o]) - lp)))
         loss = fold(_add, _f(0), generate(ids.shape, term))
