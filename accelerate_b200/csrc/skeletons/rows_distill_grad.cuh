@@ -1,7 +1,9 @@
 // Gradient of the distillation loss (rows_stats.cuh) with respect to the student's logits:
 //   ds_j = g tau (p_j - sum of q_k over the entries k with id_k = j),   p_j = e^(s_j/tau - lse),
 // 0 for a row without teacher entries.  One read and one write of the row; the normaliser comes from the forward
-// pass.  ROW_C CTAs share a row, each with a stretch of its blocks; once a CTA has written its stretch it rewrites the
+// pass.  It is one Float: half a step of it, 2^-24 of its size, is a relative error of every p_j (2^-11 at 2^14).  From
+// there on every CTA reads its row twice more, for the maximum m and Z = sum e^((s - m)/tau), and takes
+// p_j = e^((s_j - m)/tau) / Z, if these give the normaliser it got, up to three of its steps.  ROW_C CTAs share a row, each with a stretch of its blocks; once a CTA has written its stretch it rewrites the
 // elements in it that have teacher entries (an id that occurs twice is written once, with the sum).
 
 struct Params { i64 x, ids, teacher, lse, g, out, rows, n, k, tau, err; };
@@ -67,10 +69,44 @@ extern "C" __global__ void __launch_bounds__(ROW_THREADS, ROW_MIN_BLOCKS) acc_ro
   if (bad && tid == 0 && part == 0) acc_fail(p.err, 1003);
 
   // p_j g tau = 2^(c (s - tau lse)) g tau: the product tau lse is not rounded before the subtraction, so the exponent
-  // is right to half a step whatever the logits' size.  A row without an element above -inf comes with lse = -inf:
+  // is right to half a step for the lse that was given.  A row without an element above -inf comes with lse = -inf:
   // the type's lowest value in its place lets its -inf elements yield 0.
-  const f32 lse_tau = lse == -ROW_INF ? -3.402823466e38f : lse;
-#define DG_P(s) (row_ex2(fmaf(-lse_tau, tau, s) * c) * scale)
+  f32 from = lse == -ROW_INF ? -3.402823466e38f : lse, by = tau, p_scale = scale;
+  if (has && fabsf(lse) >= 16384.0f) {
+    f32 m = -ROW_INF, z = 0.0f;
+    for (int i = tid; i < span.blocks; i += ROW_THREADS) {
+      f32 v[ROW_E];
+      row_unpack(span.load(i), v);
+#pragma unroll
+      for (int e = 0; e < ROW_E; ++e) m = fmaxf(m, v[e]);
+    }
+    m = row_warp_max(m);
+    if (lane == 0) red[0][warp] = m;     // (everybody has read what was there: a barrier lies between)
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < DG_WARPS; ++w) m = fmaxf(m, red[0][w]);
+    if (m != -ROW_INF)
+      for (int i = tid; i < span.blocks; i += ROW_THREADS) {
+        f32 v[ROW_E], sum = 0.0f;
+        row_unpack(span.load(i), v);
+#pragma unroll
+        for (int e = 0; e < ROW_E; ++e) sum += row_ex2((v[e] - m) * c);
+        z += sum;
+      }
+    z = row_warp_sum(z);
+    if (lane == 0) red[1][warp] = z;
+    __syncthreads();
+    z = 0.0f;
+#pragma unroll
+    for (int w = 0; w < DG_WARPS; ++w) z += red[1][w];
+    const f32 own = m / tau + logf(z);
+    if (z > 0.0f && (own == lse || fabsf(own - lse) <= fabsf(lse) * (3.0f / 8388608.0f))) {
+      from = m;
+      by = 1.0f;
+      p_scale = scale / z;
+    }
+  }
+#define DG_P(s) (row_ex2(fmaf(-from, by, s) * c) * p_scale)
   for (int t = b0; t < b1; t += DG_TILE) {
     uint4 cur[ROW_U];
 #pragma unroll

@@ -22,6 +22,8 @@ __all__ = ["logProbs", "distill", "distillGrad", "layerNorm", "layerNormGrad"]
 
 _REAL = ("f16", "f32")
 _NONE = 2 ** 31 - 1                      # an index behind every row
+# distillGrad: a normaliser of this size is too coarse, and so near (relative) is the row's own
+_NORMALISER_LARGE, _NORMALISER_STEPS = 2.0 ** 14, 3 * 2.0 ** -23
 
 
 def _foreign(name, consts, fallback, *args):
@@ -202,7 +204,13 @@ def distillGrad(tau, ids, teacher, student, normaliser, gradient):
     ``distillGrad :: Float -> Array (sh:.Int) Int32 -> Array (sh:.Int) t' -> Array (sh:.Int) t -> Array sh Float -> Array sh Float -> Array (sh:.Int) t``
 
     ``normaliser`` is ``distill``'s second result, ``gradient`` that of the whole with respect to every row's loss; the
-    result is gradient tau (p - q), rounded once to the student's type."""
+    result is gradient tau (p - q), p = e^(student / tau - normaliser), rounded once to the student's type.
+
+    The normaliser is one Float, and half a step of it is a relative error of every p: 2^-24 of its size, so up to 2^-10
+    (with what ``distill`` rounded on the way) below 2^14.  From 2^14 on, where logits this large, small temperatures or rows
+    of the type's lowest value lead, p comes from the row itself, p = e^((student - max) / tau) / Z, as long as the given
+    normaliser is the row's own, up to three steps of it; another one (that of a longer row, of which this is a part) is taken
+    as it is."""
     ids, teacher, student, normaliser, gradient = use(ids), use(teacher), use(student), use(normaliser), use(gradient)
     _check_distill("distillGrad", tau, ids, teacher, student)
     for a in (normaliser, gradient):
@@ -211,6 +219,7 @@ def distillGrad(tau, ids, teacher, student, normaliser, gradient):
     def definition(ids, ts, xs, lse, g):
         r = xs.rank
         _, total, e = _teacher(tau, ids, ts)
+        own, top, z = _normaliser(tau, xs)
 
         def share(ix):                   # sh :. n :. k: what entry k asks for element j
             o, j = index(*[ix[d] for d in range(r - 1)]), ix[r - 1]
@@ -220,7 +229,11 @@ def distillGrad(tau, ids, teacher, student, normaliser, gradient):
 
         def one(ix):
             o = _outer(ix, r)
-            p = cond(_wide(xs[ix]).eq(_f(-math.inf)), _f(0), exp(_wide(xs[ix]) / _f(tau) - lse[o]))
+            size = abs(lse[o])
+            close = lor(lse[o].eq(own[o]), abs(lse[o] - own[o]) <= size * _f(_NORMALISER_STEPS))
+            from_row = land(land(size >= _f(_NORMALISER_LARGE), z[o] > _f(0)), close)
+            p = cond(_wide(xs[ix]).eq(_f(-math.inf)), _f(0),
+                     cond(from_row, exp((_wide(xs[ix]) - top[o]) / _f(tau)) / z[o], exp(_wide(xs[ix]) / _f(tau) - lse[o])))
             return _as(cond(total[o].eq(_f(0)), _f(0), g[o] * _f(tau) * (p - asked[ix] / total[o])), xs.elt)
         return generate(xs.shape, one)
     return _foreign("b200.distillGrad", [float(tau)], definition, ids, teacher, student, normaliser, gradient)

@@ -64,6 +64,31 @@ def check_distill(tau, ids, te, x, got, adds):
     close(loss, want, bound, "loss")
 
 
+def check_distill_grad(tau, ids, te, x, lse, g, got, adds):
+    """The gradient behind `distill`, whose normaliser `lse` it was given: tau g (softmax(x / tau) - q) of the logits
+    themselves.  A normaliser below 2^14 is taken as it is, with what its rounding does to every probability."""
+    t, ln_z, m = parts(x, tau)
+    q = teacher_q(tau, ids, te)
+    p = np.where(ln_z[..., None] == -np.inf, 0.0, np.exp(t - np.where(np.isfinite(ln_z), ln_z, 0.0)[..., None]))
+    asked = np.zeros(x.shape)
+    for r in range(x.shape[0]):
+        for i in range(ids.shape[1]):
+            if ids[r, i] >= 0:
+                asked[r, ids[r, i]] += q[r, i]
+    scale = (g.astype(np.float64) * tau)[..., None]
+    want = np.where((q.sum(-1) > 0)[..., None], scale * (p - asked), 0.0)
+    tt = np.where(ids < 0, -np.inf, te.astype(np.float64) / tau)
+    with np.errstate(invalid="ignore"):
+        far = np.max(np.where(q > 0, np.max(tt, -1, keepdims=True, initial=-np.inf) - tt, 0.0), -1, initial=0.0)[..., None]
+    with np.errstate(invalid="ignore", over="ignore"):
+        rounded = np.where(np.abs(lse) < 2.0 ** 14, U * (np.abs(m) + 3 * np.abs(lse)), 0.0)
+    off = (ln_z_bound(t, ln_z, adds) + rounded)[..., None] + U * (16 + 5 * np.where(np.isfinite(t), np.abs(t), 0.0))
+    bound = np.abs(scale) * (p * off + asked * U * (2 * ids.shape[-1] + 40 + 6 * far) + 2.0 ** -126)
+    ty = "f16" if x.dtype == np.float16 else "f32"
+    assert got.dtype == x.dtype
+    close(got, want, bound * (1 + 2.0 ** -10) + half_step(want, ty), "gradient")
+
+
 def rows_with_a_constant(g, rows, n, t, offset):
     """Logits around `offset`, in steps that the type holds there."""
     return (np.clip(g.normal(size=(rows, n)) * 6, -40, 40) + offset).astype(NP[t])
@@ -72,4 +97,4 @@ def rows_with_a_constant(g, rows, n, t, offset):
 LOWEST = {"f16": np.float16(-65504), "f32": np.finfo(np.float32).min}
 OFFSETS = [("f16", 1000.0), ("f16", -60000.0), ("f32", 1e4), ("f32", -3e6), ("f32", 2e8)]
 
-__all__ = ["parts", "ln_z_bound", "check_log_probs", "check_distill", "rows_with_a_constant", "LOWEST", "OFFSETS", "half_step"]
+__all__ = ["parts", "ln_z_bound", "check_log_probs", "check_distill", "check_distill_grad", "rows_with_a_constant", "LOWEST", "OFFSETS", "half_step"]
