@@ -82,9 +82,10 @@ class ProgramCache:
 
 
 class _View:
-    """One leaf of a device array, described the way torch takes other libraries' device memory."""
+    """One leaf of a device array, described the way torch takes other libraries' device memory.  A tensor's storage holds
+    this object as long as there are aliases of it, and this object the array."""
 
-    __slots__ = ("__cuda_array_interface__",)
+    __slots__ = ("__cuda_array_interface__", "array")
 
 
 _as_tensor = torch.as_tensor
@@ -146,10 +147,9 @@ class GpuExecutor:
             dt = np.dtype(L.NP_OF[a.leaf_types[leaf]])
             return torch.empty(a.shape, dtype=torch.from_numpy(np.empty(0, dt)).dtype, device=self.stream.device)
         v = _View()
+        v.array = a
         v.__cuda_array_interface__ = {"shape": shape or (1,), "typestr": _TYPESTR[a.leaf_types[leaf]], "data": (a.devptr(leaf), False), "version": 3}
-        t = _as_tensor(v, device=self.device)
-        t._keepalive = a
-        return t
+        return _as_tensor(v, device=self.device)
 
     def wrap(self, t, elt):
         """Device array over a torch tensor's memory (the tensor must stay alive).  Arrays are dense, so the tensor

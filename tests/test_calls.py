@@ -62,3 +62,41 @@ def test_a_result_that_is_an_input_asks_again_once_the_input_was_given_other_dat
     after, = ctx.execute("p", [a], 1)
     library.now = 333
     assert after.devptr() == 222, "known from the run"
+
+
+class Array:
+    """What `GpuExecutor.tensor` looks at of a device array."""
+
+    shape, leaf_types = (3,), ["f32"]
+
+    def devptr(self, leaf=0):
+        return 4096
+
+
+def test_what_torch_keeps_of_a_view_keeps_the_array(monkeypatch):
+    """A tensor's storage, and with it every alias (detach, a view of another type, a slice in inference mode), holds the
+    object that described the memory, not the attributes of the tensor that was made first."""
+    import gc
+    import weakref
+
+    import torch
+
+    from accelerate_b200 import sharded
+    held = []
+
+    def as_tensor(v, device):
+        held.append(v)
+        assert v.__cuda_array_interface__["data"] == (4096, False)
+        return torch.zeros(3)
+    monkeypatch.setattr(sharded, "_as_tensor", as_tensor)
+    ex = sharded.GpuExecutor.__new__(sharded.GpuExecutor)
+    ex.device = torch.device("cpu")
+    a = Array()
+    alive = weakref.ref(a)
+    t = ex.tensor(a)
+    del a, t
+    gc.collect()
+    assert alive() is not None, "the array's memory went back to the pool under a tensor that still points at it"
+    held.clear()
+    gc.collect()
+    assert alive() is None

@@ -19,3 +19,35 @@ def test_a_view_of_a_result_that_is_an_input_sees_the_adopted_payload(gpu_ctx):
     gpu_ctx.sync()
     assert view.tolist() == [7.0] * 5
     assert np.array_equal(more.download(), np.ones(5, np.float32))
+
+
+@pytest.mark.parametrize("alias", ["detach", "data", "view", "slice", "inference slice"])
+def test_an_alias_of_a_view_keeps_the_array(gpu_ctx, alias):
+    import gc
+    import weakref
+
+    import torch
+    ex = sharded.GpuExecutor(gpu_ctx)
+    x = A.param(1, "f32")
+    prog = A.build_program([A.map(lambda v: v + 1, x)])
+    out, = gpu_ctx.execute(prog.text, [gpu_ctx.from_host(np.zeros(64, np.float32))], 1)
+    gpu_ctx.sync()
+    alive = weakref.ref(out)
+    first = ex.tensor(out)
+    del out
+    if alias == "inference slice":
+        with torch.inference_mode():
+            other = first[3:]
+    else:
+        other = {"detach": lambda t: t.detach(), "data": lambda t: t.data, "view": lambda t: t.view(torch.int32), "slice": lambda t: t[3:]}[alias](first)
+    del first
+    gc.collect()
+    assert alive() is not None
+    # (the next result of this size does not get that memory)
+    again, = gpu_ctx.execute(prog.text, [gpu_ctx.from_host(np.full(64, 9, np.float32))], 1)
+    gpu_ctx.sync()
+    assert again.devptr() != alive().devptr()
+    assert other.view(torch.float32).tolist() == [1.0] * other.numel()
+    del other
+    gc.collect()
+    assert alive() is None
