@@ -5,6 +5,7 @@
 #include <Python.h>
 
 #include <cstdint>
+#include <string>
 #include <vector>
 
 namespace {
@@ -18,8 +19,8 @@ const char* (*f_error)();
 PyObject* error_class;      // B200Error(code, message)
 PyObject* type_names;       // scalar types in the library's order
 
-PyObject* fail(int rc) {
-  PyObject* args = Py_BuildValue("(is)", rc, f_error());
+PyObject* fail(int rc, const char* message) {
+  PyObject* args = Py_BuildValue("(is)", rc, message);
   if (args) {
     PyErr_SetObject(error_class, args);
     Py_DECREF(args);
@@ -30,18 +31,29 @@ bool to_u64(PyObject* o, uint64_t* v) {
   *v = PyLong_AsUnsignedLongLong(o);
   return !(*v == (uint64_t)-1 && PyErr_Occurred());
 }
-// rank, extents and leaves of an array as (shape, leaf types)
+// One result of a run, as the library describes it
+struct Result {
+  uint64_t id = 0;
+  int rank = 0, leaves = 0;
+  std::vector<int64_t> shape;
+  std::vector<int32_t> types;
+  std::vector<void*> ptrs;
+};
 constexpr int kRank = 1024, kLeaves = 1 << 16;
-bool describe(void* ctx, uint64_t id, int* rank, std::vector<int64_t>& shape, int* leaves, std::vector<int32_t>& types, int* rc) {
-  shape.resize(8);
-  types.resize(32);
-  *rc = f_info(ctx, id, 8, rank, shape.data(), 32, leaves, types.data());
-  if (*rc) {
-    shape.resize(kRank);
-    types.resize(kLeaves);
-    *rc = f_info(ctx, id, kRank, rank, shape.data(), kLeaves, leaves, types.data());
+int describe(void* ctx, Result& r) {
+  r.shape.resize(8);
+  r.types.resize(32);
+  int rc = f_info(ctx, r.id, 8, &r.rank, r.shape.data(), 32, &r.leaves, r.types.data());
+  if (rc) {
+    r.shape.resize(kRank);
+    r.types.resize(kLeaves);
+    rc = f_info(ctx, r.id, kRank, &r.rank, r.shape.data(), kLeaves, &r.leaves, r.types.data());
   }
-  return *rc == 0;
+  for (int l = 0; !rc && l < r.leaves; ++l) {
+    r.ptrs.push_back(nullptr);
+    rc = f_devptr(ctx, r.id, l, &r.ptrs.back());
+  }
+  return rc;
 }
 
 // setup(wrap, run, info, devptr, free, last_error, error class, type names)
@@ -90,7 +102,7 @@ PyObject* wrap(PyObject*, PyObject* const* args, Py_ssize_t n) {
       Py_BEGIN_ALLOW_THREADS
       rc = f_wrap((void*)ctx, elt, (int)sh.size() - 1, sh.data(), p.data(), &id);
       Py_END_ALLOW_THREADS
-      r = rc ? fail(rc) : PyLong_FromUnsignedLongLong(id);
+      r = rc ? fail(rc, f_error()) : PyLong_FromUnsignedLongLong(id);
     }
   }
   Py_XDECREF(shape);
@@ -109,53 +121,59 @@ PyObject* execute(PyObject*, PyObject* const* args, Py_ssize_t n) {
   PyObject* seq = PySequence_Fast(args[2], "ids are a sequence");
   if (!seq) return nullptr;
   std::vector<uint64_t> ins((size_t)PySequence_Fast_GET_SIZE(seq) + 1), outs((size_t)n_out + 1);
+  std::vector<Result> results((size_t)n_out);
   const int n_in = (int)ins.size() - 1;
   bool ok = true;
   for (int i = 0; ok && i < n_in; ++i) ok = to_u64(PySequence_Fast_GET_ITEM(seq, i), &ins[i]);
   Py_DECREF(seq);
   if (!ok) return nullptr;
+  // Everything that takes the context's lock, in one stretch without the interpreter's: another thread may hold the
+  // former for as long as a download takes, and wait for the latter.
   int rc;
+  std::string error;
+  auto release = [&] { for (long k = 0; k < n_out; ++k) f_free((void*)ctx, outs[k]); };
   Py_BEGIN_ALLOW_THREADS
   rc = f_run((void*)prog, ins.data(), n_in, outs.data(), (int)n_out);
+  if (rc) {
+    error = f_error();
+  } else {
+    for (long k = 0; !rc && k < n_out; ++k) {
+      results[k].id = outs[k];
+      rc = describe((void*)ctx, results[k]);
+    }
+    if (rc) {
+      error = f_error();
+      release();                         // (nobody else knows the results' ids)
+    }
+  }
   Py_END_ALLOW_THREADS
-  if (rc) return fail(rc);
-  // (on any failure from here on the results are released again: nobody else knows their ids)
+  if (rc) return fail(rc, error.c_str());
   PyObject* list = PyList_New(n_out);
-  std::vector<int64_t> shape;
-  std::vector<int32_t> types;
   for (long k = 0; list && k < n_out; ++k) {
-    int rank = 0, leaves = 0;
-    std::vector<void*> ptr;
-    bool good = describe((void*)ctx, outs[k], &rank, shape, &leaves, types, &rc);
-    for (int l = 0; good && l < leaves; ++l) {
-      ptr.push_back(nullptr);
-      good = (rc = f_devptr((void*)ctx, outs[k], l, &ptr.back())) == 0;
+    const Result& r = results[k];
+    PyObject *item = nullptr, *sh = PyTuple_New(r.rank), *ty = PyList_New(r.leaves), *pt = PyTuple_New(r.leaves);
+    for (int d = 0; sh && d < r.rank; ++d) PyTuple_SET_ITEM(sh, d, PyLong_FromLongLong(r.shape[d]));
+    for (int l = 0; ty && pt && l < r.leaves; ++l) {
+      PyObject* name = PyTuple_GetItem(type_names, r.types[l]);
+      Py_XINCREF(name);
+      PyList_SET_ITEM(ty, l, name);
+      PyTuple_SET_ITEM(pt, l, PyLong_FromVoidPtr(r.ptrs[l]));
     }
-    PyObject* item = nullptr;
-    if (!good) {
-      fail(rc);
-    } else {
-      PyObject *sh = PyTuple_New(rank), *ty = PyList_New(leaves), *pt = PyTuple_New(leaves);
-      for (int d = 0; sh && d < rank; ++d) PyTuple_SET_ITEM(sh, d, PyLong_FromLongLong(shape[d]));
-      for (int l = 0; ty && pt && l < leaves; ++l) {
-        PyObject* name = PyTuple_GetItem(type_names, types[l]);
-        Py_XINCREF(name);
-        PyList_SET_ITEM(ty, l, name);
-        PyTuple_SET_ITEM(pt, l, PyLong_FromVoidPtr(ptr[l]));
-      }
-      if (sh && ty && pt && !PyErr_Occurred()) item = Py_BuildValue("(KOOO)", (unsigned long long)outs[k], sh, ty, pt);
-      Py_XDECREF(sh);
-      Py_XDECREF(ty);
-      Py_XDECREF(pt);
-    }
+    if (sh && ty && pt && !PyErr_Occurred()) item = Py_BuildValue("(KOOO)", (unsigned long long)r.id, sh, ty, pt);
+    Py_XDECREF(sh);
+    Py_XDECREF(ty);
+    Py_XDECREF(pt);
     if (!item) {
       Py_CLEAR(list);
       break;
     }
     PyList_SET_ITEM(list, k, item);
   }
-  if (!list)
-    for (long k = 0; k < n_out; ++k) f_free((void*)ctx, outs[k]);
+  if (!list) {
+    Py_BEGIN_ALLOW_THREADS
+    release();
+    Py_END_ALLOW_THREADS
+  }
   return list;
 }
 

@@ -100,3 +100,54 @@ def test_what_torch_keeps_of_a_view_keeps_the_array(monkeypatch):
     held.clear()
     gc.collect()
     assert alive() is None
+
+
+COUNTER = r"""
+import ctypes, importlib.machinery, importlib.util, sys, threading, time
+
+path, which = sys.argv[1:]
+spec = importlib.util.spec_from_loader("_binding", importlib.machinery.ExtensionFileLoader("_binding", path))
+binding = importlib.util.module_from_spec(spec)
+spec.loader.exec_module(binding)
+libc = ctypes.CDLL(None)
+address = lambda f: ctypes.cast(f, ctypes.c_void_p).value
+# Stand-ins from the C library for what may wait for a context's lock: usleep(context), which succeeds after 0.4 s, and
+# abs(x), which succeeds at once for 0 and fails for anything else (a failed description: the results are freed again).
+wait, done = address(libc.usleep), address(libc.abs)
+calls = {name: done for name in ("wrap", "run", "info", "devptr", "free")}
+calls["free" if which == "cleanup" else which] = wait
+binding.setup(calls["wrap"], calls["run"], calls["info"], calls["devptr"], calls["free"], address(libc.gnu_get_libc_version), RuntimeError, ("f32",))
+# (a run's first argument is the program, the others' the context)
+ctx, prog = (0, 400000) if which == "run" else (400000, 0)
+call = {"cleanup": lambda: fails(lambda: binding.execute(ctx, prog, [], 1)), "wrap": lambda: binding.wrap(ctx, b"f32", (), ()), "free": lambda: binding.free(ctx, 1)}.get(which, lambda: binding.execute(ctx, prog, [], 1))
+def fails(f):
+    try:
+        f()
+        sys.exit("no error")
+    except RuntimeError:
+        pass
+
+
+thread = threading.Thread(target=call)
+longest, last = 0.0, time.perf_counter()
+began = last
+thread.start()
+while thread.is_alive():
+    time.sleep(0.001)
+    now = time.perf_counter()
+    longest, last = max(longest, now - last), now
+print(longest, last - began)
+"""
+
+
+@pytest.mark.parametrize("which", ["wrap", "run", "info", "free", "cleanup"])
+def test_the_interpreter_runs_while_a_call_waits_for_the_library(lib_built, which):
+    """A call may wait for a context's lock as long as another thread's download takes; other threads go on meanwhile."""
+    import subprocess
+    import sys
+
+    from accelerate_b200 import build
+    r = subprocess.run([sys.executable, "-c", COUNTER, build.BINDING, which], capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0, r.stderr
+    longest, whole = map(float, r.stdout.split())
+    assert whole >= 0.39 and longest < 0.3, "the interpreter stood still for as long as the call waited"
