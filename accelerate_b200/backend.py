@@ -305,10 +305,11 @@ class Context:
         return DeviceArray(self, _fast.wrap(self.handle, _SCALAR_TEXT[elt], shape, (ptr,)), elt, shape, [elt])
 
     def wrap(self, elt, shape, ptrs):
-        """Adopt caller-owned device memory (one pointer per leaf)."""
+        """Adopt caller-owned device memory (one pointer per leaf: a number or a ``ctypes.c_void_p``)."""
         if len(ptrs) != len(_leaf_types(elt)):
             raise ValueError("one pointer per scalar leaf of the element type")
         shape = tuple(map(int, shape))
+        ptrs = [p.value if isinstance(p, ctypes.c_void_p) else p for p in ptrs]
         return DeviceArray(self, _fast.wrap(self.handle, _elt_text(elt), shape, ptrs), elt, shape)
 
     # programs ---------------------------------------------------------------

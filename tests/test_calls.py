@@ -151,3 +151,11 @@ def test_the_interpreter_runs_while_a_call_waits_for_the_library(lib_built, whic
     assert r.returncode == 0, r.stderr
     longest, whole = map(float, r.stdout.split())
     assert whole >= 0.39 and longest < 0.3, "the interpreter stood still for as long as the call waited"
+
+
+def test_pointers_may_be_numbers_or_void_pointers(calls):
+    ctx, _, fast = calls
+    a = ctx.wrap(("f32", "i32"), (2,), [ctypes.c_void_p(64), 128])
+    b = ctx.wrap("f32", [np.int64(0)], (ctypes.c_void_p(None),))
+    assert a.shape == (2,) and b.shape == (0,)
+    assert [ptrs for _, _, ptrs in fast.wrapped] == [(64, 128), (None,)], "the compiled binding takes numbers and None"
