@@ -5,6 +5,7 @@
 #include <Python.h>
 
 #include <cstdint>
+#include <cstring>
 #include <string>
 #include <vector>
 
@@ -20,7 +21,9 @@ PyObject* error_class;      // B200Error(code, message)
 PyObject* type_names;       // scalar types in the library's order
 
 PyObject* fail(int rc, const char* message) {
-  PyObject* args = Py_BuildValue("(is)", rc, message);
+  // (a message may quote what the caller passed: any bytes)
+  PyObject* text = PyUnicode_DecodeUTF8(message, (Py_ssize_t)strlen(message), "replace");
+  PyObject* args = text ? Py_BuildValue("(iN)", rc, text) : nullptr;
   if (args) {
     PyErr_SetObject(error_class, args);
     Py_DECREF(args);

@@ -159,3 +159,38 @@ def test_pointers_may_be_numbers_or_void_pointers(calls):
     b = ctx.wrap("f32", [np.int64(0)], (ctypes.c_void_p(None),))
     assert a.shape == (2,) and b.shape == (0,)
     assert [ptrs for _, _, ptrs in fast.wrapped] == [(64, 128), (None,)], "the compiled binding takes numbers and None"
+
+
+MESSAGE = r"""
+import ctypes, importlib.machinery, importlib.util, sys
+
+spec = importlib.util.spec_from_loader("_binding", importlib.machinery.ExtensionFileLoader("_binding", sys.argv[1]))
+binding = importlib.util.module_from_spec(spec)
+spec.loader.exec_module(binding)
+text = ctypes.create_string_buffer(b"unknown name \xff")
+last_error = ctypes.CFUNCTYPE(ctypes.c_void_p)(lambda: ctypes.addressof(text))
+address = lambda f: ctypes.cast(f, ctypes.c_void_p).value
+a = address(ctypes.CDLL(None).abs)
+
+
+class Error(RuntimeError):
+    pass
+
+
+binding.setup(a, a, a, a, a, address(last_error), Error, ("f32",))
+for call in (lambda: binding.wrap(3, b"f32", (), ()), lambda: binding.execute(0, 3, [], 1)):
+    try:
+        call()
+        sys.exit("no error")
+    except Error as e:
+        assert e.args == (3, "unknown name �"), e.args
+"""
+
+
+def test_a_message_that_is_not_utf8_arrives_all_the_same(lib_built):
+    import subprocess
+    import sys
+
+    from accelerate_b200 import build
+    r = subprocess.run([sys.executable, "-c", MESSAGE, build.BINDING], capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0, r.stderr
