@@ -90,6 +90,7 @@ class _View:
 
 _as_tensor = torch.as_tensor
 _TYPESTR = {t: np.dtype(d).str for t, d in L.NP_OF.items()}
+_DTYPE = {t: torch.from_numpy(np.empty(0, d)).dtype for t, d in L.NP_OF.items()}
 
 
 class GpuExecutor:
@@ -152,13 +153,27 @@ class GpuExecutor:
         return _as_tensor(v, device=self.device)
 
     def wrap(self, t, elt):
-        """Device array over a torch tensor's memory (the tensor must stay alive).  Arrays are dense, so the tensor
-        must be contiguous."""
-        if not t.is_contiguous():
-            raise ValueError("only a contiguous tensor can be an array's memory")
-        a = self.ctx.wrap_scalars(elt, tuple(t.shape), t.data_ptr()) if isinstance(elt, str) and elt in L.NP_OF else self.ctx.wrap(elt, tuple(t.shape), [t.data_ptr()])
+        """Device array over a torch tensor's memory (the tensor must stay alive).  Arrays are dense and on this GPU, so
+        the tensor must be contiguous and on the context's device (or in pinned host memory), and its elements must have
+        the size of ``elt``'s and, where both are floating, be of that type; whole numbers may stand for any bits."""
+        scalar = isinstance(elt, str)
+        if not (scalar and t.dtype is _DTYPE.get(elt) and t.get_device() == self.ctx.device and t.is_contiguous()):
+            self._check_memory(t, elt)
+        a = self.ctx.wrap_scalars(elt, tuple(t.shape), t.data_ptr()) if scalar and elt in L.NP_OF else self.ctx.wrap(elt, tuple(t.shape), [t.data_ptr()])
         a._keepalive = t
         return a
+
+    def _check_memory(self, t, elt):
+        leaves = L.flatten_ty(elt)
+        dtype = _DTYPE.get(leaves[0]) if len(leaves) == 1 else None
+        if dtype is None:
+            raise ValueError(f"a tensor cannot be the memory of an array of {elt}")
+        if t.element_size() != dtype.itemsize or t.dtype.is_complex or (t.dtype.is_floating_point and dtype.is_floating_point and t.dtype != dtype):
+            raise ValueError(f"a tensor of {t.dtype} cannot be the memory of an array of {elt}")
+        if t.get_device() != self.ctx.device and t.numel() and not (t.get_device() < 0 and t.is_pinned()):
+            raise ValueError(f"only a tensor on device {self.ctx.device} can be an array's memory")
+        if not t.is_contiguous():
+            raise ValueError("only a contiguous tensor can be an array's memory")
 
     def empty(self, elt, shape):
         return self.ctx.array(elt, tuple(shape))

@@ -194,3 +194,38 @@ def test_a_message_that_is_not_utf8_arrives_all_the_same(lib_built):
     from accelerate_b200 import build
     r = subprocess.run([sys.executable, "-c", MESSAGE, build.BINDING], capture_output=True, text=True, timeout=60)
     assert r.returncode == 0, r.stderr
+
+
+class Tensor:
+    """What `GpuExecutor.wrap` looks at of a tensor."""
+
+    def __init__(self, dtype, device=0, shape=(4, 6), contiguous=True, pinned=False):
+        self.dtype, self.device_index, self.shape, self.contiguous, self.pinned = dtype, device, shape, contiguous, pinned
+
+    def get_device(self): return self.device_index
+    def element_size(self): return self.dtype.itemsize
+    def numel(self): return int(np.prod(self.shape))
+    def is_contiguous(self): return self.contiguous
+    def is_pinned(self): return self.pinned
+    def data_ptr(self): return 4096
+
+
+def test_memory_that_cannot_be_the_array_is_not_wrapped(calls):
+    import torch
+
+    from accelerate_b200 import sharded
+    ctx, _, fast = calls
+    ex = sharded.GpuExecutor.__new__(sharded.GpuExecutor)
+    ex.ctx = ctx
+    for t, elt in [(Tensor(torch.float32, device=-1), "f32"), (Tensor(torch.float32, device=1), "f32"),       # host memory; another GPU's
+                   (Tensor(torch.float16), "f32"), (Tensor(torch.int32), "i64"), (Tensor(torch.int64), "i32"),   # fewer or more bytes
+                   (Tensor(torch.bfloat16), "f16"), (Tensor(torch.complex64), "f64"),                          # other numbers
+                   (Tensor(torch.float32, contiguous=False), "f32"), (Tensor(torch.float16), ("f32",))]:
+        with pytest.raises(ValueError):
+            ex.wrap(t, elt)
+    assert not fast.wrapped
+    for t, elt in [(Tensor(torch.float32), "f32"), (Tensor(torch.bool), "u8"), (Tensor(torch.int16), "u16"), (Tensor(torch.bfloat16), "u16"),
+                   (Tensor(torch.float16), ("f16",)), (Tensor(torch.int32), "f32"),
+                   (Tensor(torch.float32, device=-1, pinned=True), "f32"), (Tensor(torch.float32, device=-1, shape=(0, 3)), "f32")]:
+        assert ex.wrap(t, elt).shape == t.shape
+    assert len(fast.wrapped) == 8
