@@ -4,8 +4,8 @@
 NVRTC kernel cache, runtime, C ABI) and the text of the hand-written sm_100a
 skeletons (``csrc/skeletons/*.cuh``), which NVRTC compiles together with the
 generated scalar code at run time.  Ahead-of-time CUDA sources (``csrc/*.cu``)
-are compiled by nvcc for sm_100a and linked in.  ``_binding.so`` is the CPython module that
-makes a run's calls.
+are compiled by nvcc for sm_100a and linked in.  ``_binding.*.so`` is the CPython module
+that makes a run's calls.
 """
 from __future__ import annotations
 
@@ -18,7 +18,7 @@ import sysconfig
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "libaccb200.so")
-BINDING = os.path.join(HERE, "_binding.so")
+BINDING = os.path.join(HERE, "_binding" + sysconfig.get_config_var("EXT_SUFFIX"))      # one for every Python version
 CUDA = os.environ.get("CUDA_HOME", "/usr/local/cuda")
 NVCC_ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
@@ -58,6 +58,9 @@ def _newer(target, sources):
 def _build_binding(force, verbose):
     """The CPython module for the calls that every run makes (csrc/python/binding.cpp)."""
     src = os.path.join(CSRC, "python", "binding.cpp")
+    untagged = os.path.join(HERE, "_binding.so")
+    if os.path.exists(untagged):         # every version would load this one, whichever it was built for
+        os.remove(untagged)
     if not force and not _newer(BINDING, [src, os.path.abspath(__file__)]):
         return
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", f"-I{sysconfig.get_paths()['include']}", src, "-o", BINDING]

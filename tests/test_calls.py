@@ -229,3 +229,15 @@ def test_memory_that_cannot_be_the_array_is_not_wrapped(calls):
                    (Tensor(torch.float32, device=-1, pinned=True), "f32"), (Tensor(torch.float32, device=-1, shape=(0, 3)), "f32")]:
         assert ex.wrap(t, elt).shape == t.shape
     assert len(fast.wrapped) == 8
+
+
+def test_the_compiled_binding_is_named_after_the_interpreter(lib_built):
+    """Another Python version in the same checkout must not load a module that was built for this one."""
+    import importlib.machinery
+    import os
+
+    from accelerate_b200 import _binding, build
+    tagged = importlib.machinery.EXTENSION_SUFFIXES[0]
+    assert "cpython" in tagged and build.BINDING.endswith("_binding" + tagged)
+    assert os.path.samefile(_binding.__file__, build.BINDING)
+    assert not os.path.exists(os.path.join(os.path.dirname(build.BINDING), "_binding.so")), "any version would load that one"
