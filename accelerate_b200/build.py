@@ -14,6 +14,7 @@ import os
 import subprocess
 import sys
 import sysconfig
+import warnings
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -63,7 +64,11 @@ def _build_binding(force, verbose):
         os.remove(untagged)
     if not force and not _newer(BINDING, [src, os.path.abspath(__file__)]):
         return
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", f"-I{sysconfig.get_paths()['include']}", src, "-o", BINDING]
+    include = sysconfig.get_paths()["include"]
+    if not os.path.exists(os.path.join(include, "Python.h")):
+        warnings.warn(f"no Python.h in {include}: the backend's calls go through ctypes, which takes longer", RuntimeWarning, stacklevel=3)
+        return
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", f"-I{include}", src, "-o", BINDING]
     if verbose:
         print(" ".join(cmd))
     subprocess.check_call(cmd)

@@ -241,3 +241,80 @@ def test_the_compiled_binding_is_named_after_the_interpreter(lib_built):
     assert "cpython" in tagged and build.BINDING.endswith("_binding" + tagged)
     assert os.path.samefile(_binding.__file__, build.BINDING)
     assert not os.path.exists(os.path.join(os.path.dirname(build.BINDING), "_binding.so")), "any version would load that one"
+
+
+def test_the_library_is_built_where_python_has_no_headers(lib_built, monkeypatch, tmp_path):
+    """The C ABI has other users, and the Python layer makes the same calls through ctypes where the module is missing."""
+    from accelerate_b200 import build
+    missing = str(tmp_path / ("_binding" + ".so"))
+    monkeypatch.setattr(build, "BINDING", missing)
+    monkeypatch.setattr(build.sysconfig, "get_paths", lambda: {"include": str(tmp_path)})
+    with pytest.warns(RuntimeWarning, match="Python.h"):
+        assert build.build() == lib_built
+    assert not (tmp_path / "_binding.so").exists()
+
+
+WITHOUT = """
+import sys, warnings
+sys.modules["accelerate_b200._binding"] = None
+from accelerate_b200 import backend
+import accelerate_b200 as A
+import numpy as np
+with warnings.catch_warnings(record=True) as said:
+    warnings.simplefilter("always")
+    backend.lib()
+assert [w.category for w in said] == [RuntimeWarning], said
+text = A.build_program([A.map(lambda v: v + 1, A.param(1, "f32"))]).text
+assert "ok elementwise" in backend.compile_check(text)
+"""
+
+
+def test_the_backend_runs_without_the_compiled_binding(lib_built):
+    import subprocess
+    import sys
+    r = subprocess.run([sys.executable, "-c", WITHOUT], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, r.stderr
+
+
+def test_calls_through_ctypes_make_the_same_of_the_library(monkeypatch):
+    """The stand-in for the compiled binding against a library that answers: ids, shapes, types, pointers, errors."""
+    class Answers(Library):
+        freed = []
+
+        def b200_array_wrap(self, ctx, elt, rank, shape, ptrs, out):
+            assert ctx == 77 and elt == b"f32" and rank == 2 and list(shape[:2]) == [2, 3] and ptrs[0] == 64
+            ctypes.cast(out, ctypes.POINTER(ctypes.c_uint64))[0] = 5
+            return 0
+
+        def b200_program_run(self, prog, ins, n_in, outs, n_out):
+            assert prog == 88 and list(ins[:n_in]) == [5, 6]
+            outs[0], outs[1] = 11, 12
+            return 0
+
+        def b200_array_info(self, ctx, ident, max_rank, rank, shape, max_leaves, leaves, types):
+            ctypes.cast(rank, ctypes.POINTER(ctypes.c_int))[0] = 1
+            ctypes.cast(leaves, ctypes.POINTER(ctypes.c_int))[0] = 2
+            shape[0], types[0], types[1] = 7, 8, 2
+            return 3 if ident == self.bad else 0
+
+        def b200_array_devptr(self, ctx, ident, leaf, out):
+            ctypes.cast(out, ctypes.POINTER(ctypes.c_void_p))[0] = 1000 * ident + leaf
+            return 0
+
+        def b200_array_free(self, ctx, ident):
+            self.freed.append(ident)
+            return 0
+
+        def b200_last_error(self):
+            return b"no such array"
+    library = Answers()
+    library.bad = None
+    monkeypatch.setattr(backend, "lib", lambda: library)
+    calls = backend._CtypesCalls
+    assert calls.wrap(77, b"f32", (2, 3), (64,)) == 5
+    assert calls.execute(77, 88, [5, 6], 2) == [(11, (7,), ["f32", "i32"], (11000, 11001)), (12, (7,), ["f32", "i32"], (12000, 12001))]
+    assert calls.free(77, 11) == 0 and library.freed == [11]
+    library.bad = 12
+    with pytest.raises(backend.B200Error) as e:
+        calls.execute(77, 88, [5, 6], 2)
+    assert e.value.code == 3 and "no such array" in str(e.value) and library.freed == [11, 11, 12], "nobody else knows the results' ids"

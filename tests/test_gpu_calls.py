@@ -51,3 +51,35 @@ def test_an_alias_of_a_view_keeps_the_array(gpu_ctx, alias):
     del other
     gc.collect()
     assert alive() is None
+
+
+WITHOUT = """
+import sys, warnings
+warnings.simplefilter("ignore", RuntimeWarning)
+sys.modules["accelerate_b200._binding"] = None
+from accelerate_b200 import backend, sharded
+import accelerate_b200 as A
+import numpy as np
+import torch
+x, v = np.arange(12, dtype=np.float32).reshape(3, 4), np.ones(4, np.float32)
+y, (mean, rstd) = backend.run(list(A.layerNorm(1e-5, v, v, x)))
+assert np.array_equal(mean, x.mean(-1)) and y.shape == (3, 4)
+ex = sharded.GpuExecutor(backend.default_context())
+t = torch.arange(6, device="cuda", dtype=torch.float32)
+torch.cuda.synchronize()
+out = ex.run("twice", lambda a: A.map(lambda e: e * 2, a), [ex.wrap(t, "f32")])
+ex.sync()
+assert ex.tensor(out).tolist() == [0, 2, 4, 6, 8, 10]
+try:
+    backend.run(list(A.logProbs(1, np.array([9, 0, 0], np.int32), x)))
+    sys.exit("no error")
+except backend.B200Error as e:
+    assert e.code == 5
+"""
+
+
+def test_runs_without_the_compiled_binding(gpu_ctx):
+    import subprocess
+    import sys
+    r = subprocess.run([sys.executable, "-c", WITHOUT], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr
