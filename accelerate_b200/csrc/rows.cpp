@@ -247,20 +247,29 @@ std::vector<std::pair<std::string, Variant>> foreign_variants(const Node& n) {
   std::vector<std::pair<std::string, Variant>> v;
   const int ve = rows_arg(n).elt.s == F16 ? 8 : 4;
   auto with = [](Variant a, const char* key) { a["NORM_SUMS"] = a["NORM_COLS"] = "0"; if (*key) a[key] = "1"; return a; };
+  auto add = [&](const char* skeleton, Variant a) {
+    for (auto& b : v)
+      if (b.second == a) return;
+    v.push_back({skeleton, std::move(a)});
+  };
   switch (n.foreign) {
-    case F_LOG_PROBS: case F_DISTILL:
-      for (int c : {1, 4}) v.push_back({"rows_stats", stats_variant(c)});
+    case F_LOG_PROBS: case F_DISTILL:    // (what ctas_per_row can give)
+      for (int c : {1, 2, 4, 8}) add("rows_stats", stats_variant(c));
       break;
-    case F_DISTILL_GRAD: v.push_back({"rows_distill_grad", distill_grad_variant(1)}); break;
-    case F_LAYER_NORM:
-      for (int64_t len : {1024, 4096, 1 << 20})
-        for (int w : {ve, 2, 1}) v.push_back({"rows_norm", norm_forward_shape(len, w, 1 << 20, 148).variant()});
+    case F_DISTILL_GRAD:
+      for (int c : {1, 2, 4, 8, 16}) add("rows_distill_grad", distill_grad_variant(c));
+      break;
+    case F_LAYER_NORM:                   // (short rows to long ones, few and many)
+      for (int64_t rows : {1 << 20, 1})
+        for (int64_t len : {1024, 4096, 1 << 20})
+          for (int w : {ve, 2, 1}) add("rows_norm", norm_forward_shape(len, w, rows, 148).variant());
       break;
     case F_LAYER_NORM_GRAD:
-      for (int64_t len : {1024, 4096, 12000, 1 << 20})
-        for (int w : {ve, 2, 1}) v.push_back({"rows_norm_grad", with(norm_grad_shape(len, w, 16 / ve, 1 << 20, 148).variant(), "")});
-      v.push_back({"rows_norm_grad", with(NormShape{1, 1, 1, 1024, true}.variant(), "NORM_SUMS")});
-      v.push_back({"rows_norm_grad", with(NormShape{1, 1, 1, kThreads, true}.variant(), "NORM_COLS")});
+      for (int64_t rows : {1 << 20, 1})
+        for (int64_t len : {1024, 4096, 12000, 1 << 20})
+          for (int w : {ve, 2, 1}) add("rows_norm_grad", with(norm_grad_shape(len, w, 16 / ve, rows, 148).variant(), ""));
+      add("rows_norm_grad", with(NormShape{1, 1, 1, 1024, true}.variant(), "NORM_SUMS"));
+      add("rows_norm_grad", with(NormShape{1, 1, 1, kThreads, true}.variant(), "NORM_COLS"));
       break;
     case F_NONE: break;
   }
