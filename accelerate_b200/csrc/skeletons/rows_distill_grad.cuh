@@ -13,7 +13,6 @@ constexpr int DG_WARPS = ROW_THREADS / 32;
 
 extern "C" __global__ void __launch_bounds__(ROW_THREADS, ROW_MIN_BLOCKS) acc_rows_distill_grad(const __grid_constant__ Params p) {
   __shared__ f32 red[2][DG_WARPS];
-  __shared__ int any_bad;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const i64 row = blockIdx.x / ROW_C;
   const int part = (int)(blockIdx.x % ROW_C);

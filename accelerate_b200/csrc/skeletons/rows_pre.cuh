@@ -1,5 +1,5 @@
 // Helpers of the row operators (log probabilities, distillation, layer norm): 16-byte blocks of Half or
-// Float values, conversions, and the parameter block.  Included in front of every rows_*.cuh skeleton.
+// Float values, conversions, warp sums.  Included in front of every rows_*.cuh skeleton.
 //
 //   ROW_F16      1: the row's elements are Half, 0: Float
 //   ROW_THREADS  threads per CTA
@@ -81,7 +81,6 @@ struct row_span {
     blocks = n_ > 0 ? (shift + n_ + ROW_E - 1) / ROW_E : 0;
   }
   __device__ __forceinline__ int first(int i) const { return i * ROW_E - shift; }
-  __device__ __forceinline__ bool whole(int i) const { return first(i) >= 0 && first(i) + ROW_E <= n; }
   // Block i; elements outside the row read as -inf, which no statistic counts.  Nothing outside the row is touched.
   __device__ __forceinline__ uint4 load(int i) const {
     const int j = first(i);
