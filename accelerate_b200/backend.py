@@ -206,7 +206,9 @@ class DeviceArray:
     shape passes both; otherwise the library is asked, once."""
 
     def __init__(self, ctx, ident, elt=None, shape=None, leaf_types=None, ptrs=None):
-        self.ctx, self.id, self._ptrs, self._since = ctx, ident, ptrs, ctx.adoptions
+        self.ctx, self.id, self._ptrs = ctx, ident, ptrs
+        if ptrs is not None:
+            self._since = ctx.adoptions
         if leaf_types is not None:
             self.shape, self.leaf_types = shape, leaf_types
         elif shape is not None and elt is not None:
@@ -350,7 +352,6 @@ class Context:
         if len(ptrs) != len(_leaf_types(elt)):
             raise ValueError("one pointer per scalar leaf of the element type")
         shape = tuple(map(int, shape))
-        ptrs = [p.value if isinstance(p, ctypes.c_void_p) else p for p in ptrs]
         return DeviceArray(self, _fast.wrap(self.handle, _elt_text(elt), shape, ptrs), elt, shape)
 
     # programs ---------------------------------------------------------------

@@ -34,28 +34,33 @@ bool to_u64(PyObject* o, uint64_t* v) {
   *v = PyLong_AsUnsignedLongLong(o);
   return !(*v == (uint64_t)-1 && PyErr_Occurred());
 }
-// One result of a run, as the library describes it
+// One result of a run, as the library describes it; arrays of more dimensions or leaves than `few` take memory of their own
 struct Result {
+  Result() = default;
+  Result(const Result&) = delete;
   uint64_t id = 0;
   int rank = 0, leaves = 0;
-  std::vector<int64_t> shape;
-  std::vector<int32_t> types;
-  std::vector<void*> ptrs;
+  struct { int64_t shape[8]; int32_t types[32]; void* ptrs[32]; } few;
+  std::vector<int64_t> more_shape;
+  std::vector<int32_t> more_types;
+  std::vector<void*> more_ptrs;
+  int64_t* shape = few.shape;
+  int32_t* types = few.types;
+  void** ptrs = few.ptrs;
 };
 constexpr int kRank = 1024, kLeaves = 1 << 16;
 int describe(void* ctx, Result& r) {
-  r.shape.resize(8);
-  r.types.resize(32);
-  int rc = f_info(ctx, r.id, 8, &r.rank, r.shape.data(), 32, &r.leaves, r.types.data());
+  int rc = f_info(ctx, r.id, 8, &r.rank, r.shape, 32, &r.leaves, r.types);
   if (rc) {
-    r.shape.resize(kRank);
-    r.types.resize(kLeaves);
-    rc = f_info(ctx, r.id, kRank, &r.rank, r.shape.data(), kLeaves, &r.leaves, r.types.data());
+    r.more_shape.resize(kRank);
+    r.more_types.resize(kLeaves);
+    r.more_ptrs.resize(kLeaves);
+    r.shape = r.more_shape.data();
+    r.types = r.more_types.data();
+    r.ptrs = r.more_ptrs.data();
+    rc = f_info(ctx, r.id, kRank, &r.rank, r.shape, kLeaves, &r.leaves, r.types);
   }
-  for (int l = 0; !rc && l < r.leaves; ++l) {
-    r.ptrs.push_back(nullptr);
-    rc = f_devptr(ctx, r.id, l, &r.ptrs.back());
-  }
+  for (int l = 0; !rc && l < r.leaves; ++l) rc = f_devptr(ctx, r.id, l, &r.ptrs[l]);
   return rc;
 }
 
@@ -93,9 +98,13 @@ PyObject* wrap(PyObject*, PyObject* const* args, Py_ssize_t n) {
     for (Py_ssize_t i = 0; i < PySequence_Fast_GET_SIZE(shape); ++i) sh.push_back(PyLong_AsLongLong(PySequence_Fast_GET_ITEM(shape, i)));
     for (Py_ssize_t i = 0; i < PySequence_Fast_GET_SIZE(ptrs) && !PyErr_Occurred(); ++i) {
       PyObject* q = PySequence_Fast_GET_ITEM(ptrs, i);
-      PyObject* ix = q == Py_None ? nullptr : PyNumber_Index(q);
-      p.push_back(ix ? PyLong_AsVoidPtr(ix) : nullptr);
-      Py_XDECREF(ix);
+      p.push_back(nullptr);
+      if (q == Py_None) continue;
+      // a number, or an object that holds one (ctypes.c_void_p, whose null is None)
+      PyObject* number = PyIndex_Check(q) ? PyNumber_Index(q) : PyObject_GetAttrString(q, "value");
+      if (!number) PyErr_Format(PyExc_TypeError, "a pointer is a number, a ctypes.c_void_p or None, not %R", q);
+      if (number && number != Py_None) p.back() = PyLong_AsVoidPtr(number);
+      Py_XDECREF(number);
     }
     if (!PyErr_Occurred()) {
       uint64_t id = 0;

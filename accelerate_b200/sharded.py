@@ -156,10 +156,11 @@ class GpuExecutor:
         """Device array over a torch tensor's memory (the tensor must stay alive).  Arrays are dense and on this GPU, so
         the tensor must be contiguous and on the context's device (or in pinned host memory), and its elements must have
         the size of ``elt``'s and, where both are floating, be of that type; whole numbers may stand for any bits."""
-        scalar = isinstance(elt, str)
-        if not (scalar and t.dtype is _DTYPE.get(elt) and t.get_device() == self.ctx.device and t.is_contiguous()):
+        ctx = self.ctx
+        dtype = _DTYPE.get(elt) if isinstance(elt, str) else None
+        if t.dtype is not dtype or t.get_device() != ctx.device or not t.is_contiguous():
             self._check_memory(t, elt)
-        a = self.ctx.wrap_scalars(elt, tuple(t.shape), t.data_ptr()) if scalar and elt in L.NP_OF else self.ctx.wrap(elt, tuple(t.shape), [t.data_ptr()])
+        a = ctx.wrap(elt, tuple(t.shape), [t.data_ptr()]) if dtype is None else ctx.wrap_scalars(elt, tuple(t.shape), t.data_ptr())
         a._keepalive = t
         return a
 

@@ -153,12 +153,45 @@ def test_the_interpreter_runs_while_a_call_waits_for_the_library(lib_built, whic
     assert whole >= 0.39 and longest < 0.3, "the interpreter stood still for as long as the call waited"
 
 
-def test_pointers_may_be_numbers_or_void_pointers(calls):
-    ctx, _, fast = calls
-    a = ctx.wrap(("f32", "i32"), (2,), [ctypes.c_void_p(64), 128])
-    b = ctx.wrap("f32", [np.int64(0)], (ctypes.c_void_p(None),))
-    assert a.shape == (2,) and b.shape == (0,)
-    assert [ptrs for _, _, ptrs in fast.wrapped] == [(64, 128), (None,)], "the compiled binding takes numbers and None"
+POINTERS = r"""
+import ctypes, importlib.machinery, importlib.util, sys
+
+spec = importlib.util.spec_from_loader("_binding", importlib.machinery.ExtensionFileLoader("_binding", sys.argv[1]))
+binding = importlib.util.module_from_spec(spec)
+spec.loader.exec_module(binding)
+address = lambda f: ctypes.cast(f, ctypes.c_void_p).value
+got = []
+
+
+@ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_void_p, ctypes.c_char_p, ctypes.c_int, ctypes.POINTER(ctypes.c_int64), ctypes.POINTER(ctypes.c_void_p),
+                  ctypes.POINTER(ctypes.c_uint64))
+def wrap(ctx, elt, rank, shape, ptrs, out):
+    got.append((ctx, elt, shape[:rank], ptrs[:4]))
+    out[0] = 10
+    return 0
+
+
+a = address(ctypes.CDLL(None).abs)
+binding.setup(address(wrap), a, a, a, a, a, RuntimeError, ("f32",))
+assert binding.wrap(5, b"f32", (2, 3), [ctypes.c_void_p(64), 128, None, ctypes.c_void_p(None)]) == 10
+assert got == [(5, b"f32", [2, 3], [64, 128, None, None])], got
+for bad in (5.0, "64", ctypes.c_float(1), [64]):
+    try:
+        binding.wrap(5, b"f32", (2, 3), [bad])
+        sys.exit(repr(bad))
+    except TypeError:
+        pass
+assert len(got) == 1
+"""
+
+
+def test_pointers_may_be_numbers_or_void_pointers(lib_built):
+    import subprocess
+    import sys
+
+    from accelerate_b200 import build
+    r = subprocess.run([sys.executable, "-c", POINTERS, build.BINDING], capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0, r.stderr
 
 
 MESSAGE = r"""
