@@ -220,7 +220,7 @@ class DeviceArray:
     def devptr(self, leaf=0):
         # (the pointers a run reported hold as long as no payload was adopted since: this may be a second handle of the
         # array that adopted it, and the library copies the payload when it is asked for the pointer)
-        if self._ptrs is not None and 0 <= leaf < len(self._ptrs) and self._since == self.ctx.adoptions:
+        if self._ptrs is not None and 0 <= leaf < len(self._ptrs) and self._since is self.ctx.adoptions:
             return self._ptrs[leaf]
         return _pointer(self.ctx.h, self.id, leaf)
 
@@ -238,7 +238,7 @@ class DeviceArray:
             for k, a in enumerate(self._adopted):
                 _check(lib().b200_array_adopt_host(self.ctx.h, self.id, k, a.ctypes.data, a.nbytes))
         finally:
-            self.ctx.adoptions += 1
+            self.ctx.adoptions = object()
         return self
 
     def download(self, out=None):
@@ -287,7 +287,7 @@ class Context:
         self._programs = {}
         self._inflight = []          # views with an asynchronous download under way (kept alive until sync)
         self._interned = {}          # host payloads registered in the memory table, by key
-        self.adoptions = 0           # payloads adopted so far (DeviceArray.devptr)
+        self.adoptions = object()    # another one whenever a payload is adopted (DeviceArray.devptr)
 
     def close(self):
         if self.h:
