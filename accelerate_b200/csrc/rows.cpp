@@ -144,9 +144,9 @@ Variant stats_variant(int ctas) { return {{"ROW_THREADS", str(kStatsThreads)}, {
 Variant distill_grad_variant(int ctas) { return {{"ROW_THREADS", str(kThreads)}, {"ROW_U", "4"}, {"ROW_MIN_BLOCKS", "4"}, {"ROW_C", str(ctas)}}; }
 
 // CTAs that share a row: at least `least`, and enough to give every SM `several`, as long as each has a tile of its own.
-// The statistics take as few as fill the machine (500 rows of 50257 Floats, k = 5: 2 CTAs per row 28.7 us, 4 CTAs
-// 42 us: every CTA finds a threshold of its own); the gradient, whose CTAs are independent, four (4096 rows of
-// 131072 Halves: 372 us with one CTA per row, 357 with four, 524 with sixteen).
+// The statistics take as few as fill the machine (500 rows of 50257 Floats, k = 5: 1 CTA per row 29.8 us, 2 CTAs 28.0,
+// 4 CTAs 40.8: every CTA finds a threshold of its own); the gradient, whose CTAs are independent, four (4096 rows of
+// 131072 Halves: 363 us with one CTA per row, 348 with four, 515 with sixteen).
 int ctas_per_row(int64_t rows, int64_t n, int elt_bytes, int sms, int least, int several, int most) {
   const int64_t tiles = (n * elt_bytes + 16 * kThreads * 4 - 1) / (16 * kThreads * 4);
   int c = 1;

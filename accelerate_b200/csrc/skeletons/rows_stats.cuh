@@ -313,10 +313,11 @@ acc_rows_stats(const __grid_constant__ Params p) {
 #endif
 #if ROW_TOPK
     if (t == b0) {
-      // The first tile sets the threshold, a key that at least k elements of the tile reach and few more.  Every warp
+      // The first tile sets the threshold, a key that at least k elements of the tile reach.  Every warp
       // answers for its share of the k: with T the largest 16-bit prefix that so many of its lanes' maxima reach, it
       // takes all maxima above T and, lane by lane, as many at T as are missing; the least key among those (rounded
-      // down to the end of its block).
+      // down to the end of its block).  Few more than k reach it as long as the share is a small part of the 32 lanes; at
+      // k = 128 every lane's maximum has to, and so do about 500 of the tile's 1024 blocks.
       const int share = (k + ST_WARPS - 1) / ST_WARPS;
       const u32 pre = mc == -ROW_INF ? 0u : (st_order(mc) >> 16);
       u32 T = 0;
@@ -423,8 +424,10 @@ acc_rows_stats(const __grid_constant__ Params p) {
   }
 #if ROW_TOPK
   if (list.overflow)
-    // More blocks came than the list holds (a row in rising order): once more over the tiles since, with the list
-    // drained as often as it may fill up.
+    // More blocks came than the list holds: once more over the tiles since, with the list drained as often as it may
+    // fill up.  That takes a row in rising order, or more than 120 alternatives: the first tile of ordinary rows then lists
+    // nearly as many blocks as there is room for (k = 128: a third of the CTAs come here, and read their whole part twice).
+    // 4096 x 131072 Halves: k = 20 212 us, 64 276, 100 363, 112 442, 120 542, 124 637, 128 781.
     for (int s = drained; s < b1; s += ST_HOT) {
 #pragma unroll 1
       for (int u = 0; u < ST_HOT / ROW_THREADS; ++u) {

@@ -142,7 +142,10 @@ class GpuExecutor:
         return a.download()
 
     def tensor(self, a, leaf=0):
-        """Zero-copy torch view of one leaf of a device array."""
+        """Zero-copy torch view of one leaf of a device array, which lives as long as the view or an alias of it.  The
+        array's memory is used again, in the order of this executor's stream, as soon as the last of them is gone: that
+        stream has to have waited for work on the view that other streams still have to do (for work that only other
+        calls of this executor follow, the wait in front of the next call is early enough)."""
         shape = a.shape
         if 0 in shape:
             dt = np.dtype(L.NP_OF[a.leaf_types[leaf]])

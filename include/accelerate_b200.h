@@ -112,7 +112,8 @@ int b200_array_devptr(b200_ctx* ctx, uint64_t id, int leaf, void** ptr);
  * definition in array code.  Behind these names the library has kernels, and AFUN only gives the result's type:
  * b200.logProbs, b200.distill, b200.distillGrad, b200.layerNorm, b200.layerNormGrad (log probabilities with entropy and
  * top alternatives, distillation from a teacher's top logits, layer norm; Half or Float rows).  Their constants and
- * arguments are checked here (B200_ERR_TYPE, B200_ERR_ARG, B200_ERR_UNSUPPORTED) and their shapes by the run
+ * arguments are checked here (B200_ERR_TYPE, B200_ERR_ARG, B200_ERR_UNSUPPORTED; AFUN does not run in the place of a call
+ * that is refused, a row of Doubles for instance, whose statistics it would compute in Float) and their shapes by the run
  * (B200_ERR_BOUNDS, "shape mismatch"); a token or id behind its row's end is reported like any index out of bounds, by the
  * next download or b200_sync.  They cannot be captured into a CUDA graph (B200_ERR_UNSUPPORTED): their results come from
  * the context's pool.  Any other NAME: AFUN is applied (Interpreter.hs:217). */

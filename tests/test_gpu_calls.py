@@ -83,3 +83,23 @@ def test_runs_without_the_compiled_binding(gpu_ctx):
     import sys
     r = subprocess.run([sys.executable, "-c", WITHOUT], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stderr
+
+
+def test_the_examples_of_the_documentation(gpu_ctx):
+    """Two ways to call a row operator: on host arrays, and on torch's tensors without copies."""
+    import os
+    import re
+
+    import torch
+    text = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "README.md")).read()
+    names = {}
+    for code in re.findall(r"```python\n(.*?)```", text, re.S):
+        exec(code, names)
+    logits, tokens = torch.tensor(names["logits"], device="cuda"), torch.tensor(names["tokens"], device="cuda")
+    for _ in range(3):
+        stats, top = names["log_probs_of"](tokens, logits)
+        # (each round's results go before the next's are computed; their memory is used again)
+        got = [t.cpu().numpy() for t in stats + top]
+    want = [names[k] for k in ("logp", "normaliser", "entropy", "ids", "top")]
+    assert all(np.array_equal(a, b) for a, b in zip(got, want))
+    assert np.array_equal(got[3], np.argsort(-names["logits"].astype(np.float64), axis=-1, kind="stable")[:, :5])
