@@ -6,6 +6,8 @@
 
 #include <cstdint>
 #include <cstring>
+#include <memory>
+#include <new>
 #include <string>
 #include <vector>
 
@@ -133,7 +135,7 @@ PyObject* execute(PyObject*, PyObject* const* args, Py_ssize_t n) {
   PyObject* seq = PySequence_Fast(args[2], "ids are a sequence");
   if (!seq) return nullptr;
   std::vector<uint64_t> ins((size_t)PySequence_Fast_GET_SIZE(seq) + 1), outs((size_t)n_out + 1);
-  std::vector<Result> results((size_t)n_out);
+  std::unique_ptr<Result[]> results;     // (described once the library has accepted their number)
   const int n_in = (int)ins.size() - 1;
   bool ok = true;
   for (int i = 0; ok && i < n_in; ++i) ok = to_u64(PySequence_Fast_GET_ITEM(seq, i), &ins[i]);
@@ -149,17 +151,17 @@ PyObject* execute(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (rc) {
     error = f_error();
   } else {
-    for (long k = 0; !rc && k < n_out; ++k) {
+    results.reset(new (std::nothrow) Result[(size_t)n_out]);
+    for (long k = 0; results && !rc && k < n_out; ++k) {
       results[k].id = outs[k];
       rc = describe((void*)ctx, results[k]);
     }
-    if (rc) {
-      error = f_error();
-      release();                         // (nobody else knows the results' ids)
-    }
+    if (rc) error = f_error();
+    if (rc || !results) release();       // (nobody else knows the results' ids)
   }
   Py_END_ALLOW_THREADS
   if (rc) return fail(rc, error.c_str());
+  if (!results) return PyErr_NoMemory();
   PyObject* list = PyList_New(n_out);
   for (long k = 0; list && k < n_out; ++k) {
     const Result& r = results[k];

@@ -351,3 +351,33 @@ def test_calls_through_ctypes_make_the_same_of_the_library(monkeypatch):
     with pytest.raises(backend.B200Error) as e:
         calls.execute(77, 88, [5, 6], 2)
     assert e.value.code == 3 and "no such array" in str(e.value) and library.freed == [11, 11, 12], "nobody else knows the results' ids"
+
+
+LARGE = r"""
+import ctypes, importlib.machinery, importlib.util, resource, sys
+
+spec = importlib.util.spec_from_loader("_binding", importlib.machinery.ExtensionFileLoader("_binding", sys.argv[1]))
+binding = importlib.util.module_from_spec(spec)
+spec.loader.exec_module(binding)
+libc = ctypes.CDLL(None)
+address = lambda f: ctypes.cast(f, ctypes.c_void_p).value
+a = address(libc.abs)
+binding.setup(a, a, a, a, a, address(libc.gnu_get_libc_version), RuntimeError, ("f32",))
+before = resource.getrusage(resource.RUSAGE_SELF).ru_maxrss
+try:
+    binding.execute(0, 3, [], 1 << 20)
+    sys.exit("no error")
+except RuntimeError:
+    pass
+assert resource.getrusage(resource.RUSAGE_SELF).ru_maxrss - before < 50 << 10
+"""
+
+
+def test_a_wrong_number_of_results_costs_no_memory(lib_built):
+    """The library says that the program yields another number; nothing is described before."""
+    import subprocess
+    import sys
+
+    from accelerate_b200 import build
+    r = subprocess.run([sys.executable, "-c", LARGE, build.BINDING], capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0, r.stderr
