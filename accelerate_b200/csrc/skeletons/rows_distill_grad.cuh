@@ -3,8 +3,9 @@
 // 0 for a row without teacher entries.  One read and one write of the row; the normaliser comes from the forward
 // pass.  It is one Float: half a step of it, 2^-24 of its size, is a relative error of every p_j (2^-11 at 2^14).  From
 // there on every CTA reads its row twice more, for the maximum m and Z = sum e^((s - m)/tau), and takes
-// p_j = e^((s_j - m)/tau) / Z, if these give the normaliser it got, up to three of its steps.  ROW_C CTAs share a row, each with a stretch of its blocks; once a CTA has written its stretch it rewrites the
-// elements in it that have teacher entries (an id that occurs twice is written once, with the sum).
+// p_j = e^((s_j - m)/tau) / Z, if these give the normaliser it got, up to three of its steps.  ROW_C CTAs share a row,
+// each with a stretch of its blocks; once a CTA has written its stretch it rewrites the elements in it that have
+// teacher entries (an id that occurs twice is written once, with the sum).
 
 struct Params { i64 x, ids, teacher, lse, g, out, rows, n, k, tau, err; };
 

@@ -89,3 +89,19 @@ def test_a_normaliser_that_is_not_the_rows_own_is_taken_as_given():
     d = x.astype(np.float64) - whole.astype(np.float64)[:, None]
     p = np.exp(d)
     F.close(got, p - q, F.U * (p * (16 + 5 * np.abs(d)) + q * 200) + F.half_step(p - q, "f32") + 2.0 ** -126, "gradient")
+
+
+@pytest.mark.parametrize("tau", [1.0, 0.25])
+@pytest.mark.parametrize("t", ["f16", "f32"])
+def test_rows_of_the_highest_value_are_uniform(t, tau):
+    """(At a temperature below 1 the normaliser of such Floats is +inf, rounded.)"""
+    g = G(8)
+    rows, n = 2, 32
+    x = np.full((rows, n), -F.LOWEST[t])
+    tok = np.array([3, n - 1], np.int32)
+    F.check_log_probs(3, tok, x, RUN(A.logProbs(3, tok, x)), n)
+    ids, te = teacher(g, rows, n, 6)
+    up = np.ones(rows, np.float32)
+    got = RUN(A.distill(tau, ids, te, x))
+    F.check_distill(tau, ids, te, x, got, n)
+    F.check_distill_grad(tau, ids, te, x, got[1], up, RUN([A.distillGrad(tau, ids, te, x, got[1], up)])[0], n)
